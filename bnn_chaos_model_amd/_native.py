@@ -37,6 +37,12 @@ class BnnSketch(C.Structure):
     _fields_ = [("nseg", C.c_int32), ("reserved", C.c_int32), ("lo", C.c_float * 4), ("hi", C.c_float * 4), ("n", C.c_int32 * 4)]
 
 
+class BnnGrouped(C.Structure):
+    _fields_ = [("rows", C.c_int64), ("copies", C.c_int32), ("members", C.c_int32), ("inputs", C.c_int32), ("outputs", C.c_int32),
+                ("dtype", C.c_int32), ("gather", C.c_int32), ("scatter", C.c_int32), ("relu", C.c_int32), ("x_row", C.c_int64),
+                ("y_row", C.c_int64), ("w_member", C.c_int64), ("w_row", C.c_int64), ("order", C.c_void_p), ("offsets", C.c_void_p)]
+
+
 class NativeError(RuntimeError):
     def __init__(self, code, msg):
         super().__init__(f"bnn_chaos_hip error {code}: {msg}")
@@ -121,6 +127,19 @@ def lib():
     L.bnn_multiswag_bands_f32.argtypes = [_vp, C.POINTER(BnnGrid), _vp, _vp, _vp, _vp, C.c_int32, C.c_int32, _vp, C.c_float, C.c_uint64,
                                           C.c_int64, C.c_int64, C.c_int32, _vp, _vp, C.POINTER(BnnStats), C.c_int32, C.POINTER(BnnSketch),
                                           _vp, _vp, _vp]
+    G = C.POINTER(BnnGrouped)
+    L.bnn_group_rows_workspace_bytes.argtypes = [C.c_int64, C.c_int32]
+    L.bnn_group_rows_i32.argtypes = [_vp, C.c_int64, C.c_int32, _vp, _vp, _vp, _vp]
+    L.bnn_grouped_linear.argtypes = [G, _vp, _vp, _vp, _vp, _vp]
+    L.bnn_grouped_linear_dx_workspace_bytes.argtypes = [G]
+    L.bnn_grouped_linear_dx.argtypes = [G, _vp, _vp, _vp, _vp, _vp]
+    L.bnn_grouped_linear_dw_workspace_bytes.argtypes = [G]
+    L.bnn_grouped_linear_dw.argtypes = [G, _vp, _vp, _vp, _vp, _vp, _vp]
+    for f in (L.bnn_group_rows_workspace_bytes, L.bnn_grouped_linear_dx_workspace_bytes, L.bnn_grouped_linear_dw_workspace_bytes):
+        f.restype = C.c_size_t
+    L.bnn_relu_grad.argtypes = [_vp, C.c_int64, _vp, C.c_int64, C.c_int64, C.c_int32, C.c_int32, _vp, _vp]
+    L.bnn_quantize_rows.argtypes = [_vp, C.c_int32, C.c_int64, C.c_int32, C.c_int64, _vp, C.c_int64, _vp, _vp]
+    L.bnn_int8_linear.argtypes = [G, _vp, _vp, _vp, _vp, _vp, _vp, _vp]
     if L.bnn_abi_version() != ABI_VERSION:
         raise NativeError(-1, f"ABI version mismatch: {SO_PATH} reports {L.bnn_abi_version()}, this binding is written for {ABI_VERSION}")
     _lib = L
@@ -132,7 +151,9 @@ EXPORTS = ("bnn_abi_version", "bnn_last_error", "bnn_device_count", "bnn_param_c
            "bnn_moments_f64", "bnn_truncnorm_f32", "bnn_prior_resample_f32", "bnn_regress_f32", "bnn_group_min_f32", "bnn_quantiles_f32", "bnn_feature_pack_f64", "bnn_philox_normal_f32", "bnn_philox_raw_u32",
            "bnn_prior_table_f32", "bnn_stats_draw_f32", "bnn_multiswag_stats_f32", "bnn_sketch_bins", "bnn_sketch_update_u32",
            "bnn_sketch_quantiles_f32", "bnn_forward_lowp_f32", "bnn_multiswag_moments_f64", "bnn_multiswag_bands_f32", "bnn_feature_nn_f32", "bnn_spec_source", "bnn_plan_attach_spec",
-           "bnn_plan_spec_attached", "bnn_spec_embedded_source", "bnn_gen_params_bytes", "bnn_nonfinite_record_bytes", "bnn_nonfinite_scan_f32")
+           "bnn_plan_spec_attached", "bnn_spec_embedded_source", "bnn_gen_params_bytes", "bnn_nonfinite_record_bytes", "bnn_nonfinite_scan_f32",
+           "bnn_group_rows_workspace_bytes", "bnn_group_rows_i32", "bnn_grouped_linear", "bnn_grouped_linear_dx_workspace_bytes", "bnn_grouped_linear_dx",
+           "bnn_grouped_linear_dw_workspace_bytes", "bnn_grouped_linear_dw", "bnn_relu_grad", "bnn_quantize_rows", "bnn_int8_linear")
 
 
 def check(rc):

@@ -1,0 +1,326 @@
+// bnn_ops_grouped.hip -- rows sorted by the ensemble member that evaluates them, and the linear layer over such groups with its gradients.
+// One of the translation units of libbnn_chaos_hip.so (bnn_internal.h lists them); entry points declared in include/bnn_chaos_hip.h, kernels of
+// the products in bnn_grouped.hip.h.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <string>
+
+#include "bnn_abi_common.h"
+#include "bnn_grouped_host.h"
+
+using namespace bnn;
+
+// ---- group_rows: a stable counting sort -----------------------------------------------------------------------------------------------------
+// One wave takes 64 consecutive pairs at a time, in order: the lanes that hold the same member are found with one ballot per bit of the key, a
+// lane's place is the number of such lanes before it, and the wave's running count per member lives in LDS.  Pairs of nobody (member outside
+// [0, G)) take key G and come last.  Two sweeps over the keys: counts per (member, block), then places.
+constexpr int GROUP_CHUNK = 8192;      // pairs per workgroup
+constexpr int GROUP_MAX_MEMBERS = 4096;
+
+__device__ __forceinline__ int key_of(const int32_t* member, int64_t i, int G) {
+    const int m = member[i];
+    return m >= 0 && m < G ? m : G;
+}
+
+// counts of this workgroup's pairs: wc[wave][G + 1]
+template <int WAVES>
+__device__ __forceinline__ void count_chunk(const int32_t* member, int64_t lo, int64_t hi, int G, int32_t* wc) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, G1 = G + 1;
+    for (int i = threadIdx.x; i < WAVES * G1; i += WAVES * 64) wc[i] = 0;
+    __syncthreads();
+    constexpr int per = GROUP_CHUNK / WAVES;
+    const int64_t a = lo + wave * per, e = min(hi, a + per);
+    for (int64_t i = a + lane; i < e; i += 64) atomicAdd(&wc[wave * G1 + key_of(member, i, G)], 1);   // (whole numbers: any order gives the same counts)
+    __syncthreads();
+}
+
+template <int WAVES>
+__global__ __launch_bounds__(WAVES * 64) void bnn_group_count_kernel(const int32_t* __restrict__ member, int64_t P, int G, int32_t* __restrict__ cnt) {
+    extern __shared__ int32_t wc[];
+    const int64_t lo = (int64_t)blockIdx.x * GROUP_CHUNK, hi = min(P, lo + GROUP_CHUNK);
+    count_chunk<WAVES>(member, lo, hi, G, wc);
+    for (int g = threadIdx.x; g <= G; g += WAVES * 64) {
+        int32_t s = 0;
+        for (int w = 0; w < WAVES; ++w) s += wc[w * (G + 1) + g];
+        cnt[(int64_t)g * gridDim.x + blockIdx.x] = s;
+    }
+}
+
+// sums along a row of 64 lanes, lane by lane
+__device__ __forceinline__ int32_t wave_scan(int32_t v) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int32_t o = __shfl_up(v, d);
+        if (lane >= d) v += o;
+    }
+    return v;
+}
+
+// member g's counts over the blocks -> exclusive prefix in place, total behind the table
+__global__ __launch_bounds__(64) void bnn_group_scan_kernel(int32_t* __restrict__ cnt, int nb, int32_t* __restrict__ total) {
+    int32_t* row = cnt + (int64_t)blockIdx.x * nb;
+    int32_t carry = 0;
+    for (int b0 = 0; b0 < nb; b0 += 64) {
+        const int b = b0 + threadIdx.x;
+        const int32_t v = b < nb ? row[b] : 0, inc = wave_scan(v);
+        if (b < nb) row[b] = carry + inc - v;
+        carry += __shfl(inc, 63);
+    }
+    if (threadIdx.x == 0) total[blockIdx.x] = carry;
+}
+
+// SINGLE: one workgroup holds every pair (no count and scan launches in front)
+template <int WAVES, bool SINGLE>
+__global__ __launch_bounds__(WAVES * 64) void bnn_group_place_kernel(const int32_t* __restrict__ member, int64_t P, int G, const int32_t* __restrict__ cnt,
+                                                                     const int32_t* __restrict__ total, int nbits, int32_t* __restrict__ order,
+                                                                     int32_t* __restrict__ offsets) {
+    extern __shared__ int32_t wc[];   // [WAVES][G + 1] counts -> places, then [G + 1] member starts
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, G1 = G + 1;
+    int32_t* start = wc + WAVES * G1;
+    const int64_t lo = (int64_t)blockIdx.x * GROUP_CHUNK, hi = min(P, lo + GROUP_CHUNK);
+    count_chunk<WAVES>(member, lo, hi, G, wc);
+    for (int g = threadIdx.x; g < G1; g += WAVES * 64) {
+        int32_t s = 0;
+        if constexpr (SINGLE) for (int w = 0; w < WAVES; ++w) s += wc[w * G1 + g];
+        else s = total[g];
+        start[g] = s;
+    }
+    __syncthreads();
+    if (wave == 0) {
+        int32_t carry = 0;
+        for (int g0 = 0; g0 < G1; g0 += 64) {
+            const int g = g0 + lane;
+            const int32_t v = g < G1 ? start[g] : 0, inc = wave_scan(v);
+            if (g < G1) {
+                start[g] = carry + inc - v;
+                if (blockIdx.x == 0) offsets[g] = carry + inc - v;
+            }
+            carry += __shfl(inc, 63);
+        }
+    }
+    __syncthreads();
+    for (int g = threadIdx.x; g < G1; g += WAVES * 64) {
+        int32_t at = start[g];
+        if constexpr (!SINGLE) at += cnt[(int64_t)g * gridDim.x + blockIdx.x];
+        for (int w = 0; w < WAVES; ++w) {
+            const int32_t c = wc[w * G1 + g];
+            wc[w * G1 + g] = at;
+            at += c;
+        }
+    }
+    __syncthreads();
+    constexpr int per = GROUP_CHUNK / WAVES;
+    const int64_t a = lo + wave * per, e = min(hi, a + per);
+    for (int64_t i0 = a; i0 < e; i0 += 64) {   // (uniform per wave)
+        const int64_t i = i0 + lane;
+        const bool in = i < e;
+        const int key = in ? key_of(member, i, G) : 0;
+        uint64_t same = __ballot(in);
+        for (int b = 0; b < nbits; ++b) {
+            const uint64_t set = __ballot(in && ((key >> b) & 1));
+            same &= ((key >> b) & 1) ? set : ~set;
+        }
+        if (in) {
+            const int before = __popcll(same & ((1ull << lane) - 1));
+            const int32_t at = wc[wave * G1 + key];
+            order[at + before] = (int32_t)i;
+            if (before == 0) wc[wave * G1 + key] = at + __popcll(same);   // (every lane of the wave has read `at`: one wave runs in step)
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
+// ---- small kernels of the gradients --------------------------------------------------------------------------------------------------------
+// dx of a row that fed several (row, copy) pairs: their sum, in the copies' order
+template <typename O>
+__global__ __launch_bounds__(256) void bnn_sum_copies_kernel(const float* __restrict__ pair, int64_t rows, int copies, int K, O* __restrict__ dx) {
+    const int64_t n = rows * K;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+        const int64_t r = i / K, k = i - r * K;
+        float s = 0.0f;
+        for (int c = 0; c < copies; ++c) s += pair[(r * copies + c) * K + k];
+        dx[i] = (O)s;
+    }
+}
+
+// dW / db of the splits, added in order
+template <typename O>
+__global__ __launch_bounds__(256) void bnn_sum_splits_kernel(const float* __restrict__ part, int splits, int64_t n, O* __restrict__ out) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+        float s = 0.0f;
+        for (int c = 0; c < splits; ++c) s += part[c * n + i];
+        out[i] = (O)s;
+    }
+}
+
+// dy where the layer's output is positive (nn.ReLU's gradient: zero at zero), zero elsewhere
+template <typename T>
+__global__ __launch_bounds__(256) void bnn_relu_grad_kernel(const T* __restrict__ dy, int64_t lddy, const T* __restrict__ y, int64_t ldy, int64_t rows, int N,
+                                                            T* __restrict__ out) {
+    const int64_t n = rows * N;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+        const int64_t r = i / N, c = i - r * N;
+        out[i] = (float)y[r * ldy + c] > 0.0f ? dy[r * lddy + c] : (T)0;
+    }
+}
+
+namespace {
+
+unsigned sweep_blocks(int64_t n) { return (unsigned)std::min<int64_t>(std::max<int64_t>((n + 255) / 256, 1), 256 * 16); }
+
+int check_grouped(const bnn_grouped* q, bool int8) {
+    if (!q) return fail(BNN_ERR_INVALID, "grouped descriptor is NULL");
+    if (q->dtype < BNN_TYPE_F32 || q->dtype > BNN_TYPE_F16) return fail(BNN_ERR_INVALID, "dtype must be one of bnn_dtype");
+    if (q->rows < 0 || q->copies < 1 || q->members < 1 || q->inputs < 1 || q->outputs < 1) return fail(BNN_ERR_INVALID, "bad rows / copies / members / inputs / outputs");
+    if (q->rows > 0x7fffffffLL / q->copies) return fail(BNN_ERR_RANGE, "rows x copies must stay below 2^31");
+    if (q->inputs > (1 << 24) || q->outputs > (1 << 24) || q->members > (1 << 24)) return fail(BNN_ERR_RANGE, "members, inputs and outputs must stay below 2^24");
+    if ((q->gather || q->scatter) && q->rows && !q->order) return fail(BNN_ERR_INVALID, "gather / scatter need order");
+    return 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t bnn_group_rows_workspace_bytes(int64_t pairs, int32_t members) {
+    if (pairs <= GROUP_CHUNK || members < 1 || members > GROUP_MAX_MEMBERS) return 0;
+    const int64_t nb = (pairs + GROUP_CHUNK - 1) / GROUP_CHUNK;
+    return (size_t)(nb + 1) * (members + 1) * sizeof(int32_t);
+}
+
+int bnn_group_rows_i32(const int32_t* member, int64_t pairs, int32_t members, int32_t* order, int32_t* offsets, void* workspace, void* stream) {
+    if (pairs < 0 || members < 1) return fail(BNN_ERR_INVALID, "bad pairs / members");
+    if (members > GROUP_MAX_MEMBERS) return fail(BNN_ERR_UNSUPPORTED, "group_rows sorts by up to 4096 members");
+    if (pairs > 0x7fffffffLL) return fail(BNN_ERR_RANGE, "pairs must stay below 2^31");
+    if (!offsets || (pairs && (!member || !order))) return fail(BNN_ERR_INVALID, "NULL argument");
+    const int64_t nb = (pairs + GROUP_CHUNK - 1) / GROUP_CHUNK;
+    if (nb > 1 && !workspace) return fail(BNN_ERR_INVALID, "workspace is NULL");
+    int nbits = 1;
+    while ((members >> nbits) != 0) ++nbits;   // keys 0 .. members
+    const hipStream_t st = (hipStream_t)stream;
+    // sixteen waves while their counts fit the 160 KB of LDS, four beyond that
+    const auto launch = [&](auto waves_tag) -> int {
+        constexpr int WAVES = decltype(waves_tag)::value;
+        const size_t lds_count = (size_t)WAVES * (members + 1) * sizeof(int32_t), lds = lds_count + (size_t)(members + 1) * sizeof(int32_t);
+        if (nb <= 1) {
+            allow_big_lds<bnn_group_place_kernel<WAVES, true>>();
+            hipLaunchKernelGGL((bnn_group_place_kernel<WAVES, true>), dim3(1), dim3(WAVES * 64), lds, st, member, pairs, members, (const int32_t*)nullptr,
+                               (const int32_t*)nullptr, nbits, order, offsets);
+            HIP_TRY(hipGetLastError());
+            return 0;
+        }
+        int32_t* cnt = (int32_t*)workspace;
+        int32_t* total = cnt + nb * (members + 1);
+        allow_big_lds<bnn_group_count_kernel<WAVES>>();
+        allow_big_lds<bnn_group_place_kernel<WAVES, false>>();
+        hipLaunchKernelGGL(bnn_group_count_kernel<WAVES>, dim3((unsigned)nb), dim3(WAVES * 64), lds_count, st, member, pairs, members, cnt);
+        HIP_TRY(hipGetLastError());
+        hipLaunchKernelGGL(bnn_group_scan_kernel, dim3((unsigned)members + 1), dim3(64), 0, st, cnt, (int)nb, total);
+        HIP_TRY(hipGetLastError());
+        hipLaunchKernelGGL((bnn_group_place_kernel<WAVES, false>), dim3((unsigned)nb), dim3(WAVES * 64), lds, st, member, pairs, members, (const int32_t*)cnt,
+                           (const int32_t*)total, nbits, order, offsets);
+        HIP_TRY(hipGetLastError());
+        return 0;
+    };
+    return members < 1024 ? launch(std::integral_constant<int, 16>{}) : launch(std::integral_constant<int, 4>{});
+}
+
+int bnn_grouped_linear(const bnn_grouped* q, const void* x, const void* w, const void* bias, void* y, void* stream) {
+    if (int rc = check_grouped(q, false)) return rc;
+    if (q->rows == 0) return 0;
+    if (!x || !w || !y || !q->offsets) return fail(BNN_ERR_INVALID, "NULL argument");
+    const int es = type_size(q->dtype);
+    RowsParams p{};
+    p.x = (const char*)x; p.w = (const char*)w; p.bias = bias; p.y = (char*)y;
+    p.order = q->order; p.offsets = q->offsets;
+    p.ldx = q->x_row * es; p.w_member = q->w_member * es; p.w_row = q->w_row * es; p.ldy = q->y_row * es;
+    p.P = (int32_t)(q->rows * q->copies); p.G = q->members; p.N = q->outputs; p.K = q->inputs;
+    p.gather_div = q->gather ? q->copies : 0; p.scatter = q->scatter ? 1 : 0; p.relu = q->relu ? 1 : 0;
+    return launch_rows(q->dtype, q->dtype, false, p, (hipStream_t)stream);
+}
+
+size_t bnn_grouped_linear_dx_workspace_bytes(const bnn_grouped* q) {
+    if (!q || q->rows <= 0 || q->inputs < 1 || q->copies < 2 || !q->gather) return 0;
+    return (size_t)q->rows * q->copies * q->inputs * sizeof(float);
+}
+
+int bnn_grouped_linear_dx(const bnn_grouped* q, const void* dy, const void* w, void* dx, void* workspace, void* stream) {
+    if (int rc = check_grouped(q, false)) return rc;
+    if (q->rows == 0) return 0;
+    if (!dy || !w || !dx || !q->offsets) return fail(BNN_ERR_INVALID, "NULL argument");
+    const int es = type_size(q->dtype);
+    const bool pairs = q->gather && q->copies > 1;   // a row of x fed several pairs: their gradients meet in fp32, one rounding at the end
+    if (pairs && !workspace) return fail(BNN_ERR_INVALID, "workspace is NULL");
+    RowsParams p{};
+    p.x = (const char*)dy; p.w = (const char*)w; p.y = pairs ? (char*)workspace : (char*)dx;
+    p.order = q->order; p.offsets = q->offsets;
+    p.ldx = q->y_row * es; p.w_member = q->w_member * es; p.w_row = q->w_row * es;
+    p.ldy = pairs ? (int64_t)q->inputs * sizeof(float) : q->x_row * es;
+    p.P = (int32_t)(q->rows * q->copies); p.G = q->members; p.N = q->inputs; p.K = q->outputs;
+    p.gather_div = q->scatter ? 1 : 0; p.scatter = q->gather ? 1 : 0;
+    if (int rc = launch_rows(q->dtype, pairs ? BNN_TYPE_F32 : q->dtype, true, p, (hipStream_t)stream)) return rc;
+    if (!pairs) return 0;
+    if (q->x_row != q->inputs) return fail(BNN_ERR_INVALID, "dx of several copies must be dense");
+    const unsigned nblk = sweep_blocks(q->rows * (int64_t)q->inputs);
+    const hipStream_t st = (hipStream_t)stream;
+    if (q->dtype == BNN_TYPE_F32) hipLaunchKernelGGL(bnn_sum_copies_kernel<float>, dim3(nblk), dim3(256), 0, st, (const float*)workspace, q->rows, q->copies, q->inputs, (float*)dx);
+    else if (q->dtype == BNN_TYPE_BF16) hipLaunchKernelGGL(bnn_sum_copies_kernel<__bf16>, dim3(nblk), dim3(256), 0, st, (const float*)workspace, q->rows, q->copies, q->inputs, (__bf16*)dx);
+    else hipLaunchKernelGGL(bnn_sum_copies_kernel<_Float16>, dim3(nblk), dim3(256), 0, st, (const float*)workspace, q->rows, q->copies, q->inputs, (_Float16*)dx);
+    HIP_TRY(hipGetLastError());
+    return 0;
+}
+
+size_t bnn_grouped_linear_dw_workspace_bytes(const bnn_grouped* q) {
+    if (!q || q->rows <= 0 || q->members < 1 || q->inputs < 1 || q->outputs < 1) return 0;
+    const int s = reduce_splits(q);
+    return s > 1 ? (size_t)s * q->members * q->outputs * ((size_t)q->inputs + 1) * sizeof(float) : 0;
+}
+
+int bnn_grouped_linear_dw(const bnn_grouped* q, const void* dy, const void* x, void* dw, void* db, void* workspace, void* stream) {
+    if (int rc = check_grouped(q, false)) return rc;
+    if (!dw || !q->offsets || (q->rows && (!dy || !x))) return fail(BNN_ERR_INVALID, "NULL argument");
+    const int es = type_size(q->dtype);
+    ReduceParams p{};
+    p.x = (const char*)x; p.dy = (const char*)dy; p.dw = (char*)dw; p.db = db; p.part = (float*)workspace;
+    p.order = q->order; p.offsets = q->offsets;
+    p.ldx = q->x_row * es; p.lddy = q->y_row * es;
+    p.P = (int32_t)(q->rows * q->copies); p.G = q->members; p.N = q->outputs; p.K = q->inputs;
+    p.x_div = q->gather ? q->copies : 0; p.dy_div = q->scatter ? 1 : 0;
+    p.splits = q->rows ? reduce_splits(q) : 1;
+    if (p.splits > 1 && (!workspace || (uintptr_t)workspace % 16)) return fail(BNN_ERR_INVALID, "workspace is NULL or not 16-byte aligned");
+    if (int rc = launch_reduce(q->dtype, p, (hipStream_t)stream)) return rc;
+    if (p.splits == 1) return 0;
+    const int64_t n = (int64_t)p.G * p.N * p.K, nb = (int64_t)p.G * p.N;
+    const float* part = (const float*)workspace;
+    const hipStream_t st = (hipStream_t)stream;
+    const auto join = [&](auto tag) -> int {
+        using O = typename decltype(tag)::type;
+        hipLaunchKernelGGL(bnn_sum_splits_kernel<O>, dim3(sweep_blocks(n)), dim3(256), 0, st, part, p.splits, n, (O*)dw);
+        HIP_TRY(hipGetLastError());
+        if (db) {
+            hipLaunchKernelGGL(bnn_sum_splits_kernel<O>, dim3(sweep_blocks(nb)), dim3(256), 0, st, part + (int64_t)p.splits * n, p.splits, nb, (O*)db);
+            HIP_TRY(hipGetLastError());
+        }
+        return 0;
+    };
+    if (q->dtype == BNN_TYPE_F32) return join(Tag<float>{});
+    if (q->dtype == BNN_TYPE_BF16) return join(Tag<__bf16>{});
+    return join(Tag<_Float16>{});
+}
+
+int bnn_relu_grad(const void* dy, int64_t dy_row, const void* y, int64_t y_row, int64_t rows, int32_t N, int32_t dtype, void* out, void* stream) {
+    if (rows < 0 || N < 1 || dtype < BNN_TYPE_F32 || dtype > BNN_TYPE_F16) return fail(BNN_ERR_INVALID, "bad argument");
+    if (rows == 0) return 0;
+    if (!dy || !y || !out) return fail(BNN_ERR_INVALID, "NULL argument");
+    const unsigned nblk = sweep_blocks(rows * (int64_t)N);
+    const hipStream_t st = (hipStream_t)stream;
+    if (dtype == BNN_TYPE_F32) hipLaunchKernelGGL(bnn_relu_grad_kernel<float>, dim3(nblk), dim3(256), 0, st, (const float*)dy, dy_row, (const float*)y, y_row, rows, N, (float*)out);
+    else if (dtype == BNN_TYPE_BF16) hipLaunchKernelGGL(bnn_relu_grad_kernel<__bf16>, dim3(nblk), dim3(256), 0, st, (const __bf16*)dy, dy_row, (const __bf16*)y, y_row, rows, N, (__bf16*)out);
+    else hipLaunchKernelGGL(bnn_relu_grad_kernel<_Float16>, dim3(nblk), dim3(256), 0, st, (const _Float16*)dy, dy_row, (const _Float16*)y, y_row, rows, N, (_Float16*)out);
+    HIP_TRY(hipGetLastError());
+    return 0;
+}
+
+}  // extern "C"

@@ -11,14 +11,17 @@ SO = os.path.join(HERE, "libbnn_chaos_hip.so")
 OBJDIR = os.path.join(HERE, "build")
 # translation units (bnn_internal.h says what each holds); the forward-kernel units dominate the build time
 SRCS = ["bnn_fwd_generic.hip", "bnn_fwd_generic82.hip", "bnn_fwd_v50spec.hip", "bnn_fwd_k31.hip", "bnn_fwd_small.hip", "bnn_fwd_k41.hip", "bnn_fwd_noisy.hip", "bnn_fwd_stats.hip", "bnn_fwd_megno.hip", "bnn_fwd_lowp.hip",
-        "bnn_abi.hip", "bnn_ops_draw.hip", "bnn_ops_reduce.hip", "bnn_ops_stats.hip", "bnn_ops_features.hip", "bnn_nonfinite.hip", "bnn_tables.cpp", "bnn_generic.cpp"]
+        "bnn_gmm.hip", "bnn_abi.hip", "bnn_ops_draw.hip", "bnn_ops_reduce.hip", "bnn_ops_stats.hip", "bnn_ops_features.hip", "bnn_nonfinite.hip", "bnn_ops_grouped.hip", "bnn_ops_int8.hip", "bnn_tables.cpp", "bnn_generic.cpp"]
 HEADERS = ["bnn_layout.h", "bnn_tables.h", "bnn_internal.h", "bnn_abi_common.h", "bnn_common.hip.h", "bnn_stats.hip.h", "bnn_forward.hip.h",
-           "bnn_lowp.hip.h", "bnn_generic.h", "bnn_generic.hip.h", os.path.join("..", "..", "include", "bnn_chaos_hip.h")]
+           "bnn_lowp.hip.h", "bnn_tile.hip.h", "bnn_grouped.hip.h", "bnn_grouped_host.h", "bnn_generic.h", "bnn_generic.hip.h", os.path.join("..", "..", "include", "bnn_chaos_hip.h")]
 CFLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off", "-fno-fast-math",
           "-Wall", "-Wno-unused-variable", "-Wno-unused-but-set-variable"]
 # per-unit flags: the reduced-precision unit writes its packed arithmetic out by hand and needs the SLP vectoriser off, or the
 # compiler rebuilds convert + v_pk_fma_f32 where v_fma_mixlo/hi_f16 is wanted (bnn_lowp.hip.h, split_pair)
-UNIT_FLAGS = {"bnn_fwd_lowp.hip": ["-fno-slp-vectorize"]}
+# The linear-layer units have no use for packed fp32 arithmetic: without it the compiler does not form it from scalar code (hipcc's host pass
+# says that it does not know the feature; that is harmless).
+_NO_PACKED = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+UNIT_FLAGS = {"bnn_fwd_lowp.hip": ["-fno-slp-vectorize"], "bnn_gmm.hip": _NO_PACKED, "bnn_ops_grouped.hip": _NO_PACKED, "bnn_ops_int8.hip": _NO_PACKED}
 
 
 def hipcc():

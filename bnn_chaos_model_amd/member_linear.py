@@ -1,0 +1,323 @@
+"""Linear layers over row groups: rows sorted by the ensemble member that evaluates them, the layer of every member on its own rows (with
+gradients), and the same layer on 8-bit operands.  ops.py offers these names next to the fused forward; this file holds their checks and calls.
+
+The reference evaluates one random member per chunk of rows (figures/spock/regression.py:78-86); here a batch may mix members row by row, and a
+layer may have any width.  As everywhere: work is enqueued on torch's current stream of the operands' device, nothing synchronises, workspaces
+belong to the call (under capture: to the graph).
+"""
+import ctypes as C
+from collections import namedtuple
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _native as N
+
+_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_INT8_MAX_INPUTS = 131072   # of 32-bit sums of products of 8-bit integers
+
+# order int32 [pairs]: pair (row * copies + copy) at every grouped row; offsets int32 [members + 1]: first grouped row of every member;
+# shape: that of the member indices, (rows,) or (rows, copies)
+RowGroups = namedtuple("RowGroups", "order offsets shape")
+# values int8 [..., K], scale float32 [...]: the numbers values * scale[..., None]
+QuantRows = namedtuple("QuantRows", "values scale")
+
+
+def _gpu(t, name, dtypes):
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype not in dtypes:
+        got = f"{t.dtype} on {t.device}" if isinstance(t, torch.Tensor) else type(t).__name__
+        raise TypeError(f"{name}: expected a GPU tensor of {' / '.join(str(d) for d in dtypes)}, got {got}")
+    return t
+
+
+def _same_device(x, **tensors):
+    for name, t in tensors.items():
+        if t is not None and t.device != x.device:
+            raise ValueError(f"{name} is on {t.device}, the rows are on {x.device}")
+
+
+class _on:
+    """The operands' device current for the calls inside (one process may drive several)."""
+    __slots__ = ("ctx",)
+
+    def __init__(self, t):
+        self.ctx = None if t.device.index == N.current_device() else torch.cuda.device(t.device)
+
+    def __enter__(self):
+        if self.ctx is not None:
+            self.ctx.__enter__()
+
+    def __exit__(self, *exc):
+        if self.ctx is not None:
+            self.ctx.__exit__(*exc)
+
+
+def _stream(t):
+    return N.stream_ptr(t.device.index)
+
+
+def _workspace(nbytes, t):
+    return torch.empty(nbytes, dtype=torch.uint8, device=t.device) if nbytes else None
+
+
+def _addr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _rows2d(t):
+    """t [n, K] with its elements side by side in a row; rows may be any distance apart (a slice, an expanded row)."""
+    return t if t.shape[1] <= 1 or t.stride(1) == 1 else t.contiguous()
+
+
+def _row_stride(t):
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _layers(w):
+    """w [G, N, K]: elements side by side along K; members and output rows any distance apart (slices of the members' flat vectors)."""
+    return w if w.shape[2] <= 1 or w.stride(2) == 1 else w.contiguous()
+
+
+def group_rows(member, n_members):
+    """Sort (row, copy) pairs by ensemble member, stably -> RowGroups(order, offsets, shape).
+
+    member: int32 [rows] or [rows, copies], the member(s) that evaluate each row; values outside [0, n_members) mean nobody (padding): those
+    pairs come last, and the layers below give them zeros.  n_members <= 4096.  One launch up to 8192 pairs, three beyond."""
+    _gpu(member, "member", (torch.int32,))
+    if member.dim() not in (1, 2):
+        raise ValueError("member must be [rows] or [rows, copies]")
+    n_members = int(n_members)
+    if not 1 <= n_members <= 4096:
+        raise ValueError("n_members must lie in 1 .. 4096")
+    if member.dim() == 2 and member.shape[1] < 1:
+        raise ValueError("member must hold at least one copy per row")
+    P = member.numel()
+    if P >= 2 ** 31:
+        raise ValueError("rows x copies must stay below 2^31")
+    m = member.contiguous()
+    order = torch.empty((P,), dtype=torch.int32, device=m.device)
+    offsets = torch.empty((n_members + 1,), dtype=torch.int32, device=m.device)
+    with _on(m):
+        ws = _workspace(N.lib().bnn_group_rows_workspace_bytes(P, n_members), m)
+        N.check(N.lib().bnn_group_rows_i32(_addr(m), P, n_members, _addr(order), _addr(offsets), _addr(ws), _stream(m)))
+    return RowGroups(order, offsets, tuple(member.shape))
+
+
+def _check_groups(groups, x, G, gather, what="x"):
+    """-> (rows, copies) of the groups, after checking them against the row operand."""
+    if not isinstance(groups, RowGroups):
+        raise TypeError("groups must be the RowGroups that group_rows returns")
+    order, offsets, shape = groups
+    _gpu(order, "groups.order", (torch.int32,))
+    _gpu(offsets, "groups.offsets", (torch.int32,))
+    _same_device(x, **{"groups.order": order, "groups.offsets": offsets})
+    rows, copies = shape if len(shape) == 2 else (shape[0], 1)
+    if order.numel() != rows * copies or not order.is_contiguous() or not offsets.is_contiguous():
+        raise ValueError("groups.order must be contiguous and hold one entry per (row, copy) pair")
+    if offsets.numel() != G + 1:
+        raise ValueError(f"groups are over {offsets.numel() - 1} members, the weights over {G}")
+    want = rows if gather else rows * copies
+    if x.shape[0] != want:
+        raise ValueError(f"{what} must have {want} rows ({'the batch' if gather else 'one per grouped pair'}), got {x.shape[0]}")
+    return rows, copies
+
+
+def _out_shape(groups, n_out, scatter):
+    return (*groups.shape, n_out) if scatter else (groups.order.numel(), n_out)
+
+
+def _check_linear(x, weight, groups, bias, gather):
+    _gpu(x, "x", tuple(_TYPES))
+    _gpu(weight, "weight", (x.dtype,))
+    if x.dim() != 2 or weight.dim() != 3 or weight.shape[2] != x.shape[1] or min(weight.shape) < 1:
+        raise ValueError("x must be [rows, K] and weight [members, N, K]")
+    if max(weight.shape) > 1 << 24:
+        raise ValueError("members, inputs and outputs must stay below 2^24")
+    G, n_out, _ = weight.shape
+    if bias is not None:
+        _gpu(bias, "bias", (x.dtype,))
+        if tuple(bias.shape) != (G, n_out):
+            raise ValueError(f"bias must be [{G}, {n_out}]")
+    _same_device(x, weight=weight, bias=bias)
+    return _check_groups(groups, x, G, gather)
+
+
+def _descriptor(groups, rows, copies, dtype, weight, x_row, y_row, gather, scatter, relu=False):
+    G, n_out, n_in = weight.shape
+    return N.BnnGrouped(rows, copies, G, n_in, n_out, _TYPES[dtype], int(bool(gather)), int(bool(scatter)), int(bool(relu)), x_row, y_row,
+                        weight.stride(0) if G > 1 else 0, weight.stride(1) if n_out > 1 else n_in, _addr(groups.order), _addr(groups.offsets))
+
+
+def _linear(x, weight, groups, bias, relu, gather, scatter, rows, copies):
+    x, weight = _rows2d(x), _layers(weight)
+    bias = None if bias is None else bias.contiguous()
+    y = torch.empty(_out_shape(groups, weight.shape[1], scatter), dtype=x.dtype, device=x.device)
+    q = _descriptor(groups, rows, copies, x.dtype, weight, _row_stride(x), weight.shape[1], gather, scatter, relu)
+    with _on(x):
+        N.check(N.lib().bnn_grouped_linear(C.byref(q), _addr(x), _addr(weight), _addr(bias), _addr(y), _stream(x)))
+    return y
+
+
+def grouped_linear_grads(dy, x, weight, groups, y=None, gather=False, scatter=False, need=(True, True, True)):
+    """Gradients of grouped_linear -> (dx, dweight, dbias), each None where `need` says so.
+
+    dy: gradient of the layer's output, in its shape; y: that output, for a layer with relu=True (the gradient passes where y > 0), else None.
+    A plain function without autograd: what grouped_linear's backward calls, and what a captured HIP graph of a training step may call.
+    dweight and dbias of a member without rows are zero; sums are fp32 and do not depend on timing."""
+    rows, copies = _check_linear(x, weight, groups, None, gather)
+    G, n_out, n_in = weight.shape
+    shape = _out_shape(groups, n_out, scatter)
+    _gpu(dy, "dy", (x.dtype,))
+    if tuple(dy.shape) != shape:
+        raise ValueError(f"dy must be {list(shape)}")
+    _same_device(x, dy=dy, y=y)
+    x, weight = _rows2d(x), _layers(weight)
+    dy = _rows2d(dy.reshape(-1, n_out))
+    need_x, need_w, need_b = need
+    with _on(x):
+        L, st = N.lib(), _stream(x)
+        if y is not None:
+            _gpu(y, "y", (x.dtype,))
+            if tuple(y.shape) != shape:
+                raise ValueError(f"y must be {list(shape)}")
+            y2 = _rows2d(y.reshape(-1, n_out))
+            masked = torch.empty((dy.shape[0], n_out), dtype=x.dtype, device=x.device)
+            N.check(L.bnn_relu_grad(_addr(dy), _row_stride(dy), _addr(y2), _row_stride(y2), dy.shape[0], n_out, _TYPES[x.dtype], _addr(masked), st))
+            dy = masked
+        dx = dw = db = None
+        if need_x:
+            dx = torch.empty((x.shape[0], n_in), dtype=x.dtype, device=x.device)
+            q = _descriptor(groups, rows, copies, x.dtype, weight, n_in, _row_stride(dy), gather, scatter)
+            ws = _workspace(L.bnn_grouped_linear_dx_workspace_bytes(C.byref(q)), x)
+            N.check(L.bnn_grouped_linear_dx(C.byref(q), _addr(dy), _addr(weight), _addr(dx), _addr(ws), st))
+        if need_w or need_b:
+            dw = torch.empty((G, n_out, n_in), dtype=x.dtype, device=x.device)
+            db = torch.empty((G, n_out), dtype=x.dtype, device=x.device) if need_b else None
+            q = _descriptor(groups, rows, copies, x.dtype, weight, _row_stride(x), _row_stride(dy), gather, scatter)
+            ws = _workspace(L.bnn_grouped_linear_dw_workspace_bytes(C.byref(q)), x)
+            N.check(L.bnn_grouped_linear_dw(C.byref(q), _addr(dy), _addr(x), _addr(dw), _addr(db), _addr(ws), st))
+    return dx, dw if need_w else None, db
+
+
+class _GroupedLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, groups, relu, gather, scatter, rows, copies):
+        y = _linear(x, weight, groups, bias, relu, gather, scatter, rows, copies)
+        ctx.save_for_backward(x, weight, groups.order, groups.offsets, y if relu else None)
+        ctx.shape, ctx.gather, ctx.scatter = groups.shape, gather, scatter
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, weight, order, offsets, y = ctx.saved_tensors
+        dx, dw, db = grouped_linear_grads(dy, x, weight, RowGroups(order, offsets, ctx.shape), y, ctx.gather, ctx.scatter,
+                                          need=ctx.needs_input_grad[:3])
+        return dx, dw, db, None, None, None, None, None, None
+
+
+def grouped_linear(x, weight, groups, bias=None, relu=False, gather=False, scatter=False):
+    """y = act(W[m] x + b[m]) for every row of every member m's group; differentiable in x, weight and bias (once).
+
+    x [rows, K] float32 / bfloat16 / float16; weight [members, N, K] and bias [members, N] of the same type; groups: group_rows(...).
+    gather=True: x holds the batch's rows, each read by the member(s) its indices name; False: x [pairs, K] is already in grouped order.
+    scatter=True: y comes in the batch's order, [rows, N] or [rows, copies, N]; False: in grouped order, [pairs, N] -- so a chain of layers
+    gathers in the first, scatters in the last and permutes nothing in between.  Rows of nobody: zero.
+    x and weight may be strided as long as the elements along K are neighbours (a layer's slice of flat parameter vectors [members, d]).
+    Sums are fp32 (float32 operands: exact fp32 products), rounded once to the operands' type."""
+    rows, copies = _check_linear(x, weight, groups, bias, gather)
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
+        return _GroupedLinear.apply(x, weight, bias, groups, relu, gather, scatter, rows, copies)
+    return _linear(x, weight, groups, bias, relu, gather, scatter, rows, copies)
+
+
+def _quantize(x, pad):
+    K = x.shape[-1]
+    x2 = _rows2d(x.reshape(-1, K))
+    rows = x2.shape[0]
+    ld = (K + pad - 1) // pad * pad
+    q = torch.empty((rows, ld), dtype=torch.int8, device=x.device)
+    scale = torch.empty((rows,), dtype=torch.float32, device=x.device)
+    with _on(x):
+        N.check(N.lib().bnn_quantize_rows(_addr(x2), _TYPES[x.dtype], rows, K, _row_stride(x2), _addr(q), ld, _addr(scale), _stream(x)))
+    return q, scale
+
+
+def _check_quantize(x):
+    _gpu(x, "x", tuple(_TYPES))
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError("x must be [..., K] with K >= 1")
+    if x.shape[-1] > 1 << 24 or x.numel() // x.shape[-1] >= 2 ** 31:
+        raise ValueError("rows must stay below 2^31, their length below 2^24")
+    if torch.is_grad_enabled() and x.requires_grad:
+        raise NotImplementedError("8-bit rows have no gradient: detach x")
+
+
+def quantize_rows(x):
+    """Rows to 8-bit integers -> QuantRows(values int8 [..., K], scale float32 [...]): scale = max |x| / 127 of the row (a token, or an output
+    channel of a weight [N, K] / [members, N, K]), values = x / scale rounded half to even, exactly.  A row of zeros has scale 0; a row that holds
+    NaN or an infinity has scale NaN, so that whatever is computed from it is NaN."""
+    _check_quantize(x)
+    q, scale = _quantize(x, 1)
+    return QuantRows(q.view(x.shape), scale.view(x.shape[:-1]))
+
+
+def int8_linear(x, weight, groups=None, bias=None, relu=False, gather=False, scatter=False, dtype=None):
+    """The linear layer on 8-bit operands with a scale per row and per output channel; integer sums are exact.
+
+    x [rows, K]: float rows (quantised here: quantize_rows) or QuantRows made earlier; weight: QuantRows of [N, K] (one matrix; groups=None) or of
+    [members, N, K] with groups / gather / scatter as in grouped_linear.  bias [N] or [members, N] in the output's type `dtype` (default: x's
+    type; float32 for QuantRows).  Inference only; K <= 131072."""
+    quant = isinstance(x, QuantRows)
+    if quant:
+        xq, xs = _gpu(x.values, "x.values", (torch.int8,)), _gpu(x.scale, "x.scale", (torch.float32,))
+        rows_of = xq
+    else:
+        _check_quantize(x)
+        rows_of = x
+    dtype = dtype or (torch.float32 if quant else x.dtype)
+    if dtype not in _TYPES:
+        raise TypeError(f"dtype must be one of {[str(d) for d in _TYPES]}")
+    if not isinstance(weight, QuantRows):
+        raise TypeError("weight must be the QuantRows that quantize_rows returns")
+    wq, ws = _gpu(weight.values, "weight.values", (torch.int8,)), _gpu(weight.scale, "weight.scale", (torch.float32,))
+    want = 2 if groups is None else 3
+    if rows_of.dim() != 2 or wq.dim() != want or wq.shape[-1] != rows_of.shape[1] or min(wq.shape) < 1:
+        raise ValueError("x must be [rows, K], weight [N, K] without groups or [members, N, K] with them")
+    if wq.shape[-1] > _INT8_MAX_INPUTS:
+        raise ValueError(f"K must not exceed {_INT8_MAX_INPUTS}: the sums are 32-bit integers")
+    if max(wq.shape) > 1 << 24:
+        raise ValueError("members and outputs must stay below 2^24")
+    if tuple(ws.shape) != tuple(wq.shape[:-1]) or (quant and tuple(xs.shape) != (xq.shape[0],)):
+        raise ValueError("scales must have their values' shape without the last dimension")
+    if bias is not None:
+        _gpu(bias, "bias", (dtype,))
+        if tuple(bias.shape) != tuple(wq.shape[:-1]):
+            raise ValueError(f"bias must be {list(wq.shape[:-1])}")
+        if torch.is_grad_enabled() and bias.requires_grad:
+            raise NotImplementedError("the 8-bit layer has no gradient: detach bias")
+        bias = bias.contiguous()
+    _same_device(rows_of, weight=wq, bias=bias, **{"weight.scale": ws}, **({"x.scale": xs} if quant else {}))
+    if groups is None:
+        if gather or scatter:
+            raise ValueError("gather / scatter need groups")
+        wq, rows, copies = wq[None], rows_of.shape[0], 1
+        if rows >= 2 ** 31:
+            raise ValueError("rows must stay below 2^31")
+        shape = (rows, wq.shape[1])
+    else:
+        rows, copies = _check_groups(groups, rows_of, wq.shape[0], gather)
+        shape = _out_shape(groups, wq.shape[1], scatter)
+    if quant:
+        xq, xs = _rows2d(xq), xs.contiguous()
+    else:
+        xq, xs = _quantize(x, 16)   # (rows of whole 16-byte chunks)
+    wq, ws = _layers(wq), ws.contiguous()
+    y = torch.empty(shape, dtype=dtype, device=xq.device)
+    G, n_out, n_in = wq.shape
+    q = N.BnnGrouped(rows, copies, G, n_in, n_out, _TYPES[dtype], int(bool(gather)), int(bool(scatter)), int(bool(relu)), _row_stride(xq), n_out,
+                     wq.stride(0) if G > 1 else 0, wq.stride(1) if n_out > 1 else n_in, None if groups is None else _addr(groups.order),
+                     None if groups is None else _addr(groups.offsets))
+    with _on(xq):
+        N.check(N.lib().bnn_int8_linear(C.byref(q), _addr(xq), _addr(xs), _addr(wq), _addr(ws), _addr(bias), _addr(y), _stream(xq)))
+    return y

@@ -682,3 +682,8 @@ def multiswag_bands(x, w_avg, w2_avg, pre_D, seed_idx, sketch, st=None, nchunks=
                                             N.ptr(sketch.mom), N.stream_ptr()))
     sketch.count += J // nchunks
     return sketch
+
+
+# ---- linear layers over row groups and on 8-bit operands (member_linear.py) ----------------------------------------------------------
+from .member_linear import (QuantRows, RowGroups, group_rows, grouped_linear, grouped_linear_grads, int8_linear,  # noqa: E402,F401
+                            quantize_rows)

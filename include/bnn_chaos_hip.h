@@ -353,6 +353,51 @@ int bnn_multiswag_bands_f32(const bnn_plan* plan, const bnn_grid* grid, const fl
                             int64_t draw_id0, int64_t system_id0, int32_t draws_per_launch, float* W_workspace, float* t_workspace,
                             const bnn_stats* st, int32_t group, const bnn_sketch* sk, uint32_t* hist, double* mom, void* stream);
 
+/* ---- linear layers over row groups --------------------------------------------------------------------------------------------------
+ * The layer y = act(W[m] x + b[m]) for a batch whose rows belong to different ensemble members m (the reference evaluates one random member
+ * per chunk: figures/spock/regression.py:78-86), for any width, with its gradients, and the same layer on 8-bit operands.
+ *
+ * A PAIR is (row, copy): row i of the batch is evaluated by `copies` members, pair p = i * copies + c.  bnn_group_rows_i32 sorts the pairs by
+ * member, stably: order[r] = pair at grouped row r, offsets[m] = first grouped row of member m (offsets[members] = end of the last one's).
+ * Pairs whose member lies outside [0, members) belong to nobody and come last; their outputs and gradients are zero.  members <= 4096 there;
+ * workspace: bnn_group_rows_workspace_bytes (0: NULL is fine).
+ *
+ * bnn_grouped: rows of x / dx are x_row elements apart, rows of y / dy y_row elements; w(m, n, k) at m * w_member + n * w_row + k.
+ * gather = 1: x (and dx) holds the batch's `rows` rows and grouped row r reads row order[r] / copies; 0: it holds rows * copies rows in grouped
+ * order.  scatter = 1: y (and dy) is in pair order; 0: in grouped order.  order is a permutation of the pairs (only read with gather or
+ * scatter; entries out of range are skipped), offsets ascend; both are device pointers.  y / dx rows are written exactly once, rows between them
+ * (x_row > inputs) are not touched.  x, w, bias, y share `dtype`; sums are fp32, one rounding at the end.
+ *   bnn_grouped_linear      y  = act(W x + b), act = ReLU with relu = 1 (NaN stays NaN); bias [members, outputs] dense or NULL
+ *   bnn_grouped_linear_dx   dx = W^T dy, the copies of a row added in order (fp32 workspace: bnn_grouped_linear_dx_workspace_bytes)
+ *   bnn_grouped_linear_dw   dw [members, outputs, inputs], db [members, outputs] (or NULL), dense; zero for a member without rows.
+ *                           The result depends on the shapes only, not on timing: no atomics.
+ *   bnn_relu_grad           out[rows, N] (dense) = dy where y > 0, else 0: the gradient in front of the two above for a layer with relu = 1 */
+enum bnn_dtype { BNN_TYPE_F32 = 0, BNN_TYPE_BF16 = 1, BNN_TYPE_F16 = 2 };
+typedef struct bnn_grouped {
+    int64_t rows;
+    int32_t copies, members, inputs, outputs, dtype, gather, scatter, relu;
+    int64_t x_row, y_row, w_member, w_row;
+    const int32_t* order;
+    const int32_t* offsets;
+} bnn_grouped;
+size_t bnn_group_rows_workspace_bytes(int64_t pairs, int32_t members);
+int bnn_group_rows_i32(const int32_t* member, int64_t pairs, int32_t members, int32_t* order, int32_t* offsets, void* workspace, void* stream);
+int bnn_grouped_linear(const bnn_grouped* q, const void* x, const void* w, const void* bias, void* y, void* stream);
+size_t bnn_grouped_linear_dx_workspace_bytes(const bnn_grouped* q);
+int bnn_grouped_linear_dx(const bnn_grouped* q, const void* dy, const void* w, void* dx, void* workspace, void* stream);
+size_t bnn_grouped_linear_dw_workspace_bytes(const bnn_grouped* q);
+int bnn_grouped_linear_dw(const bnn_grouped* q, const void* dy, const void* x, void* dw, void* db, void* workspace, void* stream);
+int bnn_relu_grad(const void* dy, int64_t dy_row, const void* y, int64_t y_row, int64_t rows, int32_t N, int32_t dtype, void* out, void* stream);
+
+/* 8-bit operands.  bnn_quantize_rows: scale = max |x| / 127 of the row, q = x / scale rounded half to even -- the exact quotient's rounding,
+ * not that of a rounded reciprocal.  A row of zeros has scale 0; a row that holds NaN or +-inf has scale NaN and codes 0, so that everything
+ * computed from it is NaN.  q rows are q_row >= K bytes apart and zero behind K.
+ * bnn_int8_linear: y(r, n) = act(sum_k q(r, k) w(m, n, k) * (x_scale[row] * w_scale[m, n]) + bias[m, n]); integer sums are exact (inputs <=
+ * 131072).  q->dtype is the type of bias and y.  offsets = NULL: a dense layer (members = copies = 1). */
+int bnn_quantize_rows(const void* x, int32_t dtype, int64_t rows, int32_t K, int64_t x_row, int8_t* q, int64_t q_row, float* scale, void* stream);
+int bnn_int8_linear(const bnn_grouped* q, const int8_t* x, const float* x_scale, const int8_t* w, const float* w_scale, const void* bias, void* y,
+                    void* stream);
+
 /* Raw Philox4x32-10 blocks for known-answer tests: out[n][4] = philox(ctr = {c0+i, c1, c2, c3}, key). */
 int bnn_philox_raw_u32(uint32_t c0, uint32_t c1, uint32_t c2, uint32_t c3, uint32_t k0, uint32_t k1, int64_t n,
                        uint32_t* out, void* stream);
