@@ -14,9 +14,9 @@ int launch_rows(int dtype, int out, bool wfc, const RowsParams& p, hipStream_t s
     return f32 ? launch_rows_typed<_Float16, float, true>(p, st) : launch_rows_typed<_Float16, _Float16, true>(p, st);
 }
 
-int launch_reduce(int dtype, const ReduceParams& p, hipStream_t st) {
-    if (dtype == BNN_TYPE_F32) return launch_reduce_typed<float>(p, st);
-    return dtype == BNN_TYPE_BF16 ? launch_reduce_typed<__bf16>(p, st) : launch_reduce_typed<_Float16>(p, st);
+int launch_reduce(int dtype, const ReduceParams& p, int tile, hipStream_t st) {
+    if (dtype == BNN_TYPE_F32) return launch_reduce_typed<float>(p, tile, st);
+    return dtype == BNN_TYPE_BF16 ? launch_reduce_typed<__bf16>(p, tile, st) : launch_reduce_typed<_Float16>(p, tile, st);
 }
 
 }  // namespace bnn

@@ -19,7 +19,8 @@ struct RowsParams {            // y_r = act(W[g] x_r + b[g]) over the rows of ev
     int32_t gather_div;        // 0: x is in grouped order; c >= 1: grouped row r reads row order[r] / c of x
     int32_t scatter;           // 1: grouped row r goes to row order[r] of y
     int32_t relu;
-    int32_t nblk, tiles_n, band;
+    int32_t nblk, tiles_n, band, block_rows;
+    int32_t vec;               // N % 4 == 0 and rows of y aligned to four elements
 };
 
 struct ReduceParams {          // dW[g] = sum over rows r of member g of dy_r x_r^T;  db[g] = sum of dy_r
@@ -28,12 +29,15 @@ struct ReduceParams {          // dW[g] = sum over rows r of member g of dy_r x_
     char* dw;                  // [G, N, K]
     void* db;                  // [G, N] or null
     float* part;               // [splits, G, N, K] then [splits, G, N] when splits > 1
-    const int32_t* order;
     const int32_t* offsets;
-    int64_t ldx, lddy;
+    const int32_t* list;       // order if either operand is gathered, else offsets (read, not used)
+    uint32_t ldx, lddy;
     int32_t P, G, N, K;
-    int32_t x_div, dy_div;     // as gather_div
+    int32_t m_x, m_dy, m_list;     // -1: row r of the grouped order is row order[r] / copies of x, row order[r] of dy, list is order; 0: row r
+    uint32_t magic, shift;         // of the division by copies
     int32_t tiles_k, splits;
+    int32_t vec;                   // K % 4 == 0 and dw aligned to four elements
+    __device__ __forceinline__ unsigned by_copies(int pair) const { return __umulhi(2u * (unsigned)pair, magic) >> shift; }
 };
 
 // ---- staging ------------------------------------------------------------------------------------------------------------------------------
@@ -47,13 +51,10 @@ struct KcStage {
     int c;   // this thread's chunk of a row, in bytes
     __device__ __forceinline__ static int row_of(int i) { return (threadIdx.x + i * NT) >> 3; }
     __device__ __forceinline__ void init() { c = ((threadIdx.x & 7) ^ kc_swz(threadIdx.x >> 3)) * CHUNK; }
-    __device__ __forceinline__ void issue(char* lds, int64_t k0, int64_t kbytes) {
+    __device__ __forceinline__ void issue(char* lds, int64_t k0, int64_t kbytes, int i) {   // the i-th of its N loads
         const int64_t at = k0 + c;
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            if constexpr (DMA) load_to_lds(at < kbytes ? p[i] + at : (const char*)zero_chunk, lds + ((threadIdx.x & ~63) + i * NT) * CHUNK);
-            else r[i] = load_chunk<T>(p[i], at, kbytes);
-        }
+        if constexpr (DMA) load_to_lds(at < kbytes ? p[i] + at : (const char*)zero_chunk, lds + (__builtin_amdgcn_readfirstlane(threadIdx.x & ~63) + i * NT) * CHUNK);
+        else r[i] = load_chunk<T>(p[i], at, kbytes, k0 + STAGE_BYTES <= kbytes);
     }
     __device__ __forceinline__ void commit(char* lds) {
         if constexpr (!DMA)
@@ -62,45 +63,33 @@ struct KcStage {
     }
 };
 
-// FC operand: 128 / sizeof(T) rows of the reduction, W columns each, from column byte `col0` of rows of `width` bytes.
+// FC operand: 128 / sizeof(T) rows of the reduction per stage, W columns each, from column byte `col0` of rows of `width` bytes.  A thread's rows are
+// NT / CW apart.
 template <typename T, int W, int NT, bool DMA>
 struct FcStage {
-    static constexpr int CW = W * (int)sizeof(T) / CHUNK, N = W * 8 / NT, KR = stage_k<T>();
-    static_assert(W * 8 % NT == 0 && NT % CW == 0, "whole chunks per thread");
-    const char* base;
-    const int32_t* order;   // row k of the reduction is row order[first + k] / div of the matrix (div == 0: row first + k)
-    int64_t ld;
-    int64_t width, col0;
-    int first, limit, P, div;   // rows [first, limit); P = bound of order's values
-    int nxt[N];
+    static constexpr int CW = W * (int)sizeof(T) / CHUNK, N = W * 8 / NT, KR = stage_k<T>(), STEP = NT / CW;
+    static_assert(W * 8 % NT == 0 && NT % CW == 0 && STEP % 8 == 0, "whole chunks per thread, at most two chunk columns per thread");
+    int64_t at[2];     // byte of this thread's chunk in a row: of its even and odd loads
+    bool inside;       // all of the tile's columns are the matrix's
     u32x4 r[DMA ? 1 : N];
-    __device__ __forceinline__ static int k_of(int i) { return (threadIdx.x + i * NT) / CW; }
-    __device__ __forceinline__ int64_t col_of(int i) const { return col0 + (((int)threadIdx.x % CW) ^ fc_swz<T, W>(k_of(i))) * CHUNK; }
-    __device__ __forceinline__ void fetch(int kt) {   // the rows' places for stage kt
+    __device__ __forceinline__ static int k_of(int i) { return threadIdx.x / CW + i * STEP; }
+    __device__ __forceinline__ void init(int64_t col0, int64_t width) {
+        inside = col0 + W * (int64_t)sizeof(T) <= width;
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int row = first + kt * KR + k_of(i);
-            int src = row < limit ? row : -1;
-            if (div > 0 && src >= 0) {
-                src = order[row];
-                src = src >= 0 && src < P ? src : -1;
-            }
-            nxt[i] = src;
+        for (int o = 0; o < 2; ++o) {
+            at[o] = col0 + (((int)threadIdx.x % CW) ^ fc_swz<T, W>(k_of(o))) * CHUNK;
+            if (DMA && at[o] >= width) at[o] = 0;   // (columns behind the matrix: any, they are not stored)
         }
     }
-    __device__ __forceinline__ void issue(char* lds, int kt) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int64_t at = col_of(i);
-            const int src = div > 1 && nxt[i] >= 0 ? nxt[i] / div : nxt[i];
-            const char* row = base + (int64_t)src * ld;
-            if constexpr (DMA) load_to_lds(src < 0 ? (const char*)zero_chunk : row + (at < width ? at : 0), lds + ((threadIdx.x & ~63) + i * NT) * CHUNK);
-            else {
-                r[i] = u32x4{0, 0, 0, 0};
-                if (src >= 0) r[i] = load_chunk<T>(row, at, width);
-            }
+    __device__ __forceinline__ void issue(char* lds, const char* row, bool live, int64_t width, int i) {   // the i-th of its N loads
+        const int64_t a = at[STEP % 16 == 0 ? 0 : i & 1];
+        if constexpr (DMA) {
+            const char* src = row + a;
+            load_to_lds(live ? src : (const char*)zero_chunk, lds + (__builtin_amdgcn_readfirstlane(threadIdx.x & ~63) + i * NT) * CHUNK);
+        } else {
+            if (width >= CHUNK) r[i] = load_chunk<T>(live ? row : (const char*)zero_chunk, live ? a : 0, live ? width : CHUNK, inside);
+            else r[i] = live ? load_short<T>(row, a, width) : u32x4{0, 0, 0, 0};
         }
-        fetch(kt + 1);
     }
     __device__ __forceinline__ void commit(char* lds) {
         if constexpr (!DMA)
@@ -109,40 +98,124 @@ struct FcStage {
     }
 };
 
-template <bool DMA>
-__device__ __forceinline__ void stage_barrier() {   // this wave's loads have landed in LDS, then everybody's
-    __builtin_amdgcn_s_waitcnt(0);
-    __syncthreads();
+// ---- the loop over the reduction ----------------------------------------------------------------------------------------------------------
+// acc += first . second over KT stages of 128 bytes, two LDS buffers.  A stage is two 64-byte steps with a register set of fragments each; the
+// fragments of a step are read while the products of the step before run, across the stage border too.  Two barriers cut a stage into three parts:
+//   1  the second step's fragments are read under the first step's products;                       then nobody reads this stage's buffer any more
+//   2  the loads of the stage after next start into it, under products;                            then the next stage has landed
+//   3  the next stage's first fragments are read under the rest of the products
+// so that a load has one and a third stages to arrive.  The compiler keeps the order of loads into LDS and reads from it, so the parts are written as
+// they should issue, the products spread between.
+//   issue(kt, i)  load i of LOADS of stage kt; before(kt) comes ahead of the first; commit(kt) stores what loads through registers brought
+//   read(kt, s, i, first, second)  fragment i of F1 + F2 of step s, READS LDS reads in all
+// (stages behind the last are issued too: they read zeros into buffers that nobody reads)
+constexpr int wait_loads(int n) { return (n & 15) | 0x0f70 | (n >> 4) << 14; }   // s_waitcnt vmcnt(n)
+constexpr int WAIT_LDS = 0xc07f;                                                 // s_waitcnt lgkmcnt(0)
+
+__device__ __forceinline__ void workgroup_barrier() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+template <typename T, int F1, int F2, int READS, int LOADS, bool DMA, class Before, class Issue, class Commit, class Read>
+__device__ __forceinline__ void tile_loop(int KT, typename Mma<T>::Acc (&acc)[F1][F2], Before before, Issue issue, Commit commit, Read read) {
+    constexpr int FR = F1 + F2, PR = F1 * F2, C1 = (PR + 1) / 2, C2 = PR / 4, MF = sizeof(T) == 4 ? 4 : 1, FLY = DMA ? LOADS : 63;
+    u32x4 a0[F1], b0[F2], a1[F1], b1[F2];
+    const auto products = [&](u32x4 (&a)[F1], u32x4 (&b)[F2], int lo, int hi) {
+#pragma unroll
+        for (int j = 0; j < F1; ++j)
+#pragma unroll
+            for (int f = 0; f < F2; ++f)
+                if (j * F2 + f >= lo && j * F2 + f < hi) acc[j][f] = Mma<T>::mul(a[j], b[f], acc[j][f]);
+    };
+    before(0);
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) issue(0, i);
+    commit(0);
+    before(1);
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) issue(1, i);
+    __builtin_amdgcn_s_waitcnt(wait_loads(FLY));
+    __builtin_amdgcn_s_waitcnt(WAIT_LDS);
+    workgroup_barrier();
+#pragma unroll
+    for (int i = 0; i < FR; ++i) read(0, 0, i, a0, b0);
+    for (int kt = 0; kt + 1 < KT; ++kt) {
+        __builtin_amdgcn_s_waitcnt(WAIT_LDS);   // the fragments read in part 3, before more reads are in flight
+#pragma unroll
+        for (int i = 0; i < FR; ++i) read(kt, 1, i, a1, b1);
+        products(a0, b0, 0, C1);
+#pragma unroll
+        for (int i = 0; i < READS; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        commit(kt + 1);
+        __builtin_amdgcn_s_waitcnt(WAIT_LDS);
+        workgroup_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+        before(kt + 2);
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) issue(kt + 2, i);
+        products(a0, b0, C1, PR);
+        products(a1, b1, 0, C2);
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, (PR - C1 + C2) * MF / LOADS > 0 ? (PR - C1 + C2) * MF / LOADS : 1, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_waitcnt(wait_loads(FLY));   // all but the loads just issued (what came before them, too)
+        workgroup_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < FR; ++i) read(kt + 1, 0, i, a0, b0);
+        products(a1, b1, C2, PR);
+#pragma unroll
+        for (int i = 0; i < READS; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int i = 0; i < FR; ++i) read(KT - 1, 1, i, a1, b1);
+    products(a0, b0, 0, PR);
+    products(a1, b1, 0, PR);
+    __builtin_amdgcn_s_waitcnt(0);   // (nothing is on its way into LDS when the wave ends)
 }
 
 // ---- stores -------------------------------------------------------------------------------------------------------------------------------
+// four neighbours of a row of N, one rounding each, to nearest even, from the fp32 sums.  vec: N % 4 == 0 and rows aligned to four elements.
 template <typename O>
 __device__ __forceinline__ void store4(char* row, int n, int N, const float v[4], bool vec) {
     O* d = reinterpret_cast<O*>(row) + n;
-    if (vec && n + 4 <= N) {
-        typedef O O4 __attribute__((ext_vector_type(4)));
-        *reinterpret_cast<O4*>(d) = O4{(O)v[0], (O)v[1], (O)v[2], (O)v[3]};   // (one rounding, to nearest even, from the fp32 accumulator)
+    typedef O O4 __attribute__((ext_vector_type(4)));
+    const O4 o = {(O)v[0], (O)v[1], (O)v[2], (O)v[3]};
+    if (vec) {
+        if (n < N) *reinterpret_cast<O4*>(d) = o;
     } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            if (n + i < N) d[i] = (O)v[i];
+            if (n + i < N) d[i] = o[i];
     }
 }
 
 // ---- forward / dX --------------------------------------------------------------------------------------------------------------------------
 // BM rows x BN outputs per workgroup, WM x WN waves.  WFC: the matrix is used the other way round (element (k, n) at k * w_row + n): dX.
 template <typename T, typename O, int BM, int BN, int WM, int WN, bool WFC, bool DMA>
-__global__ __launch_bounds__(WM * WN * 64) void bnn_grouped_kernel(RowsParams p) {
+__global__ __launch_bounds__(WM * WN * 64, WM * WN * 64 >= 512 ? 2 : 1) void bnn_grouped_kernel(RowsParams p) {
     constexpr int NT = WM * WN * 64, FM = BM / WM / 16, FN = BN / WN / 16, BUF = (BM + BN) * STAGE_BYTES;
     using M = Mma<T>;
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     int tm, tn;
     tile_of_block(p.nblk, p.tiles_n, p.band, tm, tn);
-    const RowTile rt = find_rows<BM>(p.offsets, p.G, p.P, tm);
+    const RowTile rt = find_rows(p.offsets, p.G, p.P, tm, BM);
     if (rt.g < 0) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave / WN, wn = wave % WN;
     const int n0 = tn * BN;
-    const bool vec = p.N % 4 == 0 && p.ldy % (4 * sizeof(O)) == 0 && ((uintptr_t)p.y % (4 * sizeof(O))) == 0;
     auto out_row = [&](int m) -> char* {
         if (m >= rt.r1) return nullptr;
         int64_t o = m;
@@ -157,7 +230,7 @@ __global__ __launch_bounds__(WM * WN * 64) void bnn_grouped_kernel(RowsParams p)
         for (int f = 0; f < FM; ++f) {
             char* row = out_row(rt.r0 + wm * (BM / WM) + f * 16 + (lane & 15));
             if (!row) continue;
-            for (int j = 0; j < FN; ++j) store4<O>(row, n0 + wn * (BN / WN) + j * 16 + (lane >> 4) * 4, p.N, z, vec);
+            for (int j = 0; j < FN; ++j) store4<O>(row, n0 + wn * (BN / WN) + j * 16 + (lane >> 4) * 4, p.N, z, DMA || p.vec);
         }
         return;
     }
@@ -175,22 +248,24 @@ __global__ __launch_bounds__(WM * WN * 64) void bnn_grouped_kernel(RowsParams p)
         sa.p[i] = p.x + src * p.ldx;
     }
     const char* wg = p.w + rt.g * p.w_member;
+    const char* wl = wg + (int64_t)FcStage<T, BN, NT, DMA>::k_of(0) * p.w_row;
     KcStage<T, BN, NT, DMA> sb;
     FcStage<T, BN, NT, DMA> sf;
     if constexpr (WFC) {
-        sf.base = wg; sf.order = nullptr; sf.ld = p.w_row; sf.width = (int64_t)p.N * sizeof(T); sf.col0 = (int64_t)n0 * sizeof(T);
-        sf.first = 0; sf.limit = p.K; sf.P = p.K; sf.div = 0;
-        sf.fetch(0);
+        sf.init((int64_t)n0 * sizeof(T), (int64_t)p.N * sizeof(T));
     } else {
         sb.init();
 #pragma unroll
         for (int i = 0; i < sb.N; ++i) sb.p[i] = wg + (int64_t)min(n0 + sb.row_of(i), p.N - 1) * p.w_row;
     }
-    auto issue = [&](int kt) {
+    auto issue = [&](int kt, int i) {
         char* buf = smem + (kt & 1) * BUF;
-        sa.issue(buf, (int64_t)kt * STAGE_BYTES, kbytes);
-        if constexpr (WFC) sf.issue(buf + BM * STAGE_BYTES, kt);
-        else sb.issue(buf + BM * STAGE_BYTES, (int64_t)kt * STAGE_BYTES, kbytes);
+        if (i < sa.N) sa.issue(buf, (int64_t)kt * STAGE_BYTES, kbytes, i);
+        else if constexpr (WFC) {
+            const int k = kt * stage_k<T>() + (i - sa.N) * sf.STEP;   // of the wave's first rows
+            sf.issue(buf + BM * STAGE_BYTES, wl + (int64_t)k * p.w_row, k + sf.k_of(0) < p.K, (int64_t)p.N * sizeof(T), i - sa.N);
+        }
+        else sb.issue(buf + BM * STAGE_BYTES, (int64_t)kt * STAGE_BYTES, kbytes, i - sa.N);
     };
     auto commit = [&](int kt) {
         char* buf = smem + (kt & 1) * BUF;
@@ -204,31 +279,29 @@ __global__ __launch_bounds__(WM * WN * 64) void bnn_grouped_kernel(RowsParams p)
 #pragma unroll
         for (int f = 0; f < FM; ++f) acc[j][f] = typename M::Acc{};
     const int KT = (int)((kbytes + STAGE_BYTES - 1) / STAGE_BYTES);
-    issue(0);
-    commit(0);
-    for (int kt = 0; kt < KT; ++kt) {
-        stage_barrier<DMA>();
-        if (kt + 1 < KT) issue(kt + 1);
+    tile_loop<T, FN, FM, FM + FN * (WFC ? (sizeof(T) == 4 ? 4 : 2) : 1), (BM + BN) * 8 / NT, DMA>(KT, acc, [](int) {}, issue, commit,
+        [&](int kt, int st, int i, u32x4 (&fb)[FN], u32x4 (&fa)[FM]) {
         const char* a = smem + (kt & 1) * BUF;
         const char* b = a + BM * STAGE_BYTES;
+        if (i < FM) fa[i] = frag_kc<T>(a, wm * (BM / WM) + i * 16, st, lane);
+        else if constexpr (WFC) fb[i - FM] = frag_fc<T, BN>(b, wn * (BN / WN) + (i - FM) * 16, st, lane);
+        else fb[i - FM] = frag_kc<T>(b, wn * (BN / WN) + (i - FM) * 16, st, lane);
+    });
+    tf32x4 bias[FN], ws[FN];   // of this lane's four outputs per fragment (outputs behind N: not stored)
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            if (s == 1 && (int64_t)kt * STAGE_BYTES + 64 >= kbytes) break;   // nothing of the reduction in the second half
-            u32x4 fa[FM], fb[FN];
+    for (int j = 0; j < FN; ++j)
 #pragma unroll
-            for (int f = 0; f < FM; ++f) fa[f] = frag_kc<T>(a, wm * (BM / WM) + f * 16, s, lane);
-#pragma unroll
-            for (int j = 0; j < FN; ++j) {
-                if constexpr (WFC) fb[j] = frag_fc<T, BN>(b, wn * (BN / WN) + j * 16, s, lane);
-                else fb[j] = frag_kc<T>(b, wn * (BN / WN) + j * 16, s, lane);
-            }
-#pragma unroll
-            for (int j = 0; j < FN; ++j)
-#pragma unroll
-                for (int f = 0; f < FM; ++f) acc[j][f] = M::mul(fb[j], fa[f], acc[j][f]);
+        for (int i = 0; i < 4; ++i) {
+            const int64_t col = (int64_t)rt.g * p.N + min(n0 + wn * (BN / WN) + j * 16 + (lane >> 4) * 4 + i, p.N - 1);
+            bias[j][i] = 0.0f;
+            ws[j][i] = sizeof(T) == 1 ? p.ws[col] : 1.0f;
         }
-        if (kt + 1 < KT) commit(kt + 1);
-    }
+    if (p.bias)
+#pragma unroll
+        for (int j = 0; j < FN; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                bias[j][i] = (float)reinterpret_cast<const O*>(p.bias)[(int64_t)rt.g * p.N + min(n0 + wn * (BN / WN) + j * 16 + (lane >> 4) * 4 + i, p.N - 1)];
 #pragma unroll
     for (int f = 0; f < FM; ++f) {
         const int m = rt.r0 + wm * (BM / WM) + f * 16 + (lane & 15);
@@ -245,31 +318,212 @@ __global__ __launch_bounds__(WM * WN * 64) void bnn_grouped_kernel(RowsParams p)
         }
 #pragma unroll
         for (int j = 0; j < FN; ++j) {
-            const int n = n0 + wn * (BN / WN) + j * 16 + (lane >> 4) * 4;
             float v[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int64_t col = (int64_t)rt.g * p.N + min(n + i, p.N - 1);
-                if constexpr (sizeof(T) == 1) v[i] = (float)acc[j][f][i] * (xs * p.ws[col]);
-                else v[i] = acc[j][f][i];
-                if (p.bias) v[i] += (float)reinterpret_cast<const O*>(p.bias)[col];
+                v[i] = (sizeof(T) == 1 ? (float)acc[j][f][i] * (xs * ws[j][i]) : (float)acc[j][f][i]) + bias[j][i];
                 if (p.relu) v[i] = v[i] < 0.0f ? 0.0f : v[i];   // (NaN stays NaN, as in nn.ReLU)
             }
-            store4<O>(row, n, p.N, v, vec);
+            store4<O>(row, n0 + wn * (BN / WN) + j * 16 + (lane >> 4) * 4, p.N, v, DMA || p.vec);
         }
     }
 }
 
-// ---- dW, db --------------------------------------------------------------------------------------------------------------------------------
-// BN outputs x BK inputs of one member per workgroup (blockIdx.y), over split blockIdx.z of the member's rows.  The bias gradient is the same
-// product with a column of ones and falls out of the workgroups of the first input tile.
-template <typename T, typename O, int BN, int BK, int WN, int WK, bool DMA>
-__global__ __launch_bounds__(WN * WK * 64) void bnn_grouped_dw_kernel(ReduceParams p) {
-    constexpr int NT = WN * WK * 64, FN = BN / WN / 16, FK = BK / WK / 16, BUF = (BN + BK) * STAGE_BYTES, KR = stage_k<T>();
+// ---- forward of few rows --------------------------------------------------------------------------------------------------------------------
+// 16 FM rows x 16 FN outputs per workgroup of eight waves.  With few rows per member the matrices are what is read: nothing is shared through LDS,
+// every wave takes an eighth of the reduction and loads fragments of W and x as they lie in memory (64 bytes of 16 rows per load, U steps in
+// flight), and the eight partial sums meet in LDS, in the waves' order.
+template <typename T, typename O, int FM, int FN, int U, bool VEC>
+__global__ __launch_bounds__(512) void bnn_grouped_few_kernel(RowsParams p) {
+    constexpr int WAVES = 8, BM = 16 * FM, BN = 16 * FN, STEP = 64;
     using M = Mma<T>;
+    using Acc = typename M::Acc;
+    extern __shared__ __attribute__((aligned(1024))) char smem[];
+    Acc* part = reinterpret_cast<Acc*>(smem);   // [WAVES][FM * FN][64]
+    int tm, tn;
+    tile_of_block(p.nblk, p.tiles_n, p.band, tm, tn);
+    const RowTile rt = find_rows(p.offsets, p.G, p.P, tm, BM);
+    if (rt.g < 0) return;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n0 = tn * BN, q16 = (lane >> 4) * CHUNK;
+    const bool nobody = rt.g == p.G && p.offsets;
+    Acc acc[FM][FN];
+#pragma unroll
+    for (int f = 0; f < FM; ++f)
+#pragma unroll
+        for (int j = 0; j < FN; ++j) acc[f][j] = Acc{};
+    if (!nobody) {
+        const int64_t kbytes = (int64_t)p.K * sizeof(T);
+        const char *px[FM], *pw[FN];
+#pragma unroll
+        for (int f = 0; f < FM; ++f) {
+            const int m = min(rt.r0 + f * 16 + (lane & 15), rt.r1 - 1);
+            int64_t src = m;
+            if (p.gather_div) {
+                const int o = p.order[m];
+                src = o >= 0 && o < p.P ? (p.gather_div > 1 ? o / p.gather_div : o) : 0;
+            }
+            px[f] = p.x + src * p.ldx;
+        }
+#pragma unroll
+        for (int j = 0; j < FN; ++j) pw[j] = p.w + rt.g * p.w_member + (int64_t)min(n0 + j * 16 + (lane & 15), p.N - 1) * p.w_row;
+        const int steps = (int)((kbytes + STEP - 1) / STEP), per = (steps + WAVES - 1) / WAVES, end = min(steps, (wave + 1) * per);
+        const auto load = [&](const char* row, int step) -> u32x4 {   // past the wave's share or the row's end: zero
+            const int64_t at = (int64_t)step * STEP + q16;
+            if constexpr (VEC) return *reinterpret_cast<const u32x4*>(step < end && at < kbytes ? row + at : (const char*)zero_chunk);
+            else if (kbytes >= CHUNK) return step < end ? load_chunk<T>(row, at, kbytes, ((int64_t)step + 1) * STEP <= kbytes) : u32x4{0, 0, 0, 0};
+            else return load_short<T>(row, at, step < end ? kbytes : 0);
+        };
+        for (int s0 = wave * per; s0 < end; s0 += U) {
+            u32x4 w[U][FN], x[U][FM];
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int j = 0; j < FN; ++j) w[u][j] = load(pw[j], s0 + u);
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int f = 0; f < FM; ++f) x[u][f] = load(px[f], s0 + u);
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int f = 0; f < FM; ++f)
+#pragma unroll
+                    for (int j = 0; j < FN; ++j) acc[f][j] = M::mul(w[u][j], x[u][f], acc[f][j]);
+        }
+    }
+#pragma unroll
+    for (int f = 0; f < FM; ++f)
+#pragma unroll
+        for (int j = 0; j < FN; ++j) part[(wave * FM * FN + f * FN + j) * 64 + lane] = acc[f][j];
+    __syncthreads();
+    for (int t = tid; t < FM * FN * 64; t += 512) {
+        Acc a = part[t];
+        for (int w = 1; w < WAVES; ++w) a += part[w * FM * FN * 64 + t];
+        const int frag = t >> 6, l = t & 63;
+        const int m = rt.r0 + frag / FN * 16 + (l & 15), n = n0 + frag % FN * 16 + (l >> 4) * 4;
+        if (m >= rt.r1) continue;
+        int64_t o = m, src = m;
+        if (p.order && (p.scatter || p.gather_div)) {
+            const int pair = p.order[m];
+            if (pair < 0 || pair >= p.P) continue;
+            if (p.scatter) o = pair;
+            if (p.gather_div) src = pair / p.gather_div;
+        }
+        float v[4] = {0, 0, 0, 0};
+        if (!nobody) {
+            const float xs = sizeof(T) == 1 ? p.xs[src] : 1.0f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int64_t col = (int64_t)rt.g * p.N + min(n + i, p.N - 1);
+                v[i] = sizeof(T) == 1 ? (float)a[i] * (xs * p.ws[col]) : (float)a[i];
+                if (p.bias) v[i] += (float)reinterpret_cast<const O*>(p.bias)[col];
+                if (p.relu) v[i] = v[i] < 0.0f ? 0.0f : v[i];
+            }
+        }
+        store4<O>(p.y + o * p.ldy, n, p.N, v, VEC || p.vec);
+    }
+}
+
+// ---- forward of short rows ----------------------------------------------------------------------------------------------------------------
+// 16 FN outputs of up to 64 ST bytes of reduction: the member's matrix stays in FN x ST fragments of a wave's registers (at most 32: 128
+// registers) while `block_rows` rows of the batch stream by, sixteen at a time and wave by wave -- no LDS, no barrier; what is read and written
+// is the batch.  The rows' places are fetched two steps ahead and the rows one step ahead of their products.
+template <typename T, typename O, int FN, int ST>
+__global__ __launch_bounds__(256) void bnn_grouped_short_kernel(RowsParams p) {
+    constexpr int WAVES = 4, BN = 16 * FN, STEP = 64;
+    using M = Mma<T>;
+    using Acc = typename M::Acc;
+    int tm, tn;
+    tile_of_block(p.nblk, p.tiles_n, p.band, tm, tn);
+    const RowTile rt = find_rows(p.offsets, p.G, p.P, tm, p.block_rows);
+    if (rt.g < 0) return;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n0 = tn * BN, i16 = lane & 15, q = lane >> 4;
+    const bool nobody = rt.g == p.G && p.offsets;
+    const int64_t kbytes = (int64_t)p.K * sizeof(T);
+    const char* wg = p.w + (nobody ? 0 : rt.g) * p.w_member;
+    u32x4 w[FN][ST];
+    float bias[FN][4], ws[FN][4];
+#pragma unroll
+    for (int j = 0; j < FN; ++j) {
+#pragma unroll
+        for (int s = 0; s < ST; ++s) {
+            const int at = s * STEP + q * CHUNK, n = n0 + j * 16 + i16;
+            w[j][s] = load_chunk<T>(wg + (int64_t)min(n, p.N - 1) * p.w_row, at, kbytes, (s + 1) * STEP <= kbytes);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int64_t col = (int64_t)(nobody ? 0 : rt.g) * p.N + min(n0 + j * 16 + q * 4 + i, p.N - 1);
+            bias[j][i] = p.bias && !nobody ? (float)reinterpret_cast<const O*>(p.bias)[col] : 0.0f;
+            ws[j][i] = sizeof(T) == 1 ? p.ws[col] : 1.0f;
+        }
+    }
+    const bool listed = p.gather_div || p.scatter;
+    const auto place = [&](int m) -> int {   // the pair at grouped row m (m itself without an order)
+        const int r = min(m, rt.r1 - 1);
+        return listed ? p.order[r] : r;
+    };
+    const auto source = [&](int m, int pair) -> int64_t {   // row of x
+        if (!p.gather_div) return min(m, rt.r1 - 1);
+        const int o = pair >= 0 && pair < p.P ? pair : 0;
+        return p.gather_div > 1 ? o / p.gather_div : o;
+    };
+    const auto fetch = [&](int64_t src, u32x4 (&x)[ST]) {
+        const char* row = p.x + src * p.ldx;
+#pragma unroll
+        for (int s = 0; s < ST; ++s) {
+            const int at = s * STEP + q * CHUNK;
+            x[s] = load_chunk<T>(row, at, kbytes, (s + 1) * STEP <= kbytes);
+        }
+    };
+    int m = rt.r0 + wave * 16 + i16;
+    int pair = place(m), pair1 = place(m + 16 * WAVES);
+    int64_t src = source(m, pair);
+    u32x4 x[ST];
+    if (!nobody) fetch(src, x);
+    for (; m - i16 < rt.r1; m += 16 * WAVES) {
+        u32x4 xn[ST];
+        const int64_t src1 = source(m + 16 * WAVES, pair1);
+        const int pair2 = place(m + 32 * WAVES);
+        if (!nobody) fetch(src1, xn);
+        Acc acc[FN];
+#pragma unroll
+        for (int j = 0; j < FN; ++j) acc[j] = Acc{};
+        if (!nobody)
+#pragma unroll
+            for (int s = 0; s < ST; ++s)
+#pragma unroll
+                for (int j = 0; j < FN; ++j) acc[j] = M::mul(w[j][s], x[s], acc[j]);
+        const int o = p.scatter ? pair : m;
+        if (m < rt.r1 && o >= 0 && o < p.P) {
+            char* row = p.y + (int64_t)o * p.ldy;
+            const float xs = sizeof(T) == 1 && !nobody ? p.xs[src] : 1.0f;
+#pragma unroll
+            for (int j = 0; j < FN; ++j) {
+                float v[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    v[i] = (sizeof(T) == 1 ? (float)acc[j][i] * (xs * ws[j][i]) : (float)acc[j][i]) + bias[j][i];
+                    if (p.relu) v[i] = v[i] < 0.0f ? 0.0f : v[i];
+                }
+                store4<O>(row, n0 + j * 16 + q * 4, p.N, v, p.vec);
+            }
+        }
+        pair = pair1; pair1 = pair2; src = src1;
+#pragma unroll
+        for (int s = 0; s < ST; ++s) x[s] = xn[s];
+    }
+}
+
+// ---- dW, db --------------------------------------------------------------------------------------------------------------------------------
+// BT outputs x BT inputs of one member per workgroup (blockIdx.y), over split blockIdx.z of the member's rows.  The workgroups in front of the first
+// input tile sum dy's columns (the bias gradient) instead.
+template <typename T, typename O, int BT, int WN, int WK, bool DMA>
+__global__ __launch_bounds__(WN * WK * 64, WN * WK * 64 >= 512 ? 2 : 1) void bnn_grouped_dw_kernel(ReduceParams p) {
+    constexpr int NT = WN * WK * 64, FN = BT / WN / 16, FK = BT / WK / 16, BUF = 2 * BT * STAGE_BYTES, KR = stage_k<T>();
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wn = wave / WK, wk = wave % WK;
-    const int g = blockIdx.y, n0 = ((int)blockIdx.x / p.tiles_k) * BN, k0 = ((int)blockIdx.x % p.tiles_k) * BK;
+    const int cols = p.tiles_k + (p.db ? 1 : 0);
+    const int g = blockIdx.y, n0 = ((int)blockIdx.x / cols) * BT, tk = (int)blockIdx.x % cols - (p.db ? 1 : 0), k0 = tk * BT;
     int r0 = min(max(p.offsets[g], 0), p.P), r1 = min(max(p.offsets[g + 1], r0), p.P);
     if (p.splits > 1) {   // whole stages per split
         const int64_t len = (((int64_t)(r1 - r0) + p.splits - 1) / p.splits + KR - 1) / KR * KR;
@@ -278,78 +532,107 @@ __global__ __launch_bounds__(WN * WK * 64) void bnn_grouped_dw_kernel(ReducePara
         r1 = (int)(lo + len < r1 ? lo + len : r1);
         r1 = max(r1, r0);
     }
-    FcStage<T, BN, NT, DMA> sy;
-    FcStage<T, BK, NT, DMA> sx;
-    sy.base = p.dy; sy.order = p.order; sy.ld = p.lddy; sy.width = (int64_t)p.N * sizeof(T); sy.col0 = (int64_t)n0 * sizeof(T);
-    sy.first = r0; sy.limit = r1; sy.P = p.P; sy.div = p.dy_div;
-    sx.base = p.x; sx.order = p.order; sx.ld = p.ldx; sx.width = (int64_t)p.K * sizeof(T); sx.col0 = (int64_t)k0 * sizeof(T);
-    sx.first = r0; sx.limit = r1; sx.P = p.P; sx.div = p.x_div;
-    typename M::Acc acc[FK][FN], sum[FN];
-#pragma unroll
-    for (int f = 0; f < FN; ++f) {
-        sum[f] = typename M::Acc{};
-#pragma unroll
-        for (int j = 0; j < FK; ++j) acc[j][f] = typename M::Acc{};
-    }
-    const bool bias = p.db && k0 == 0 && wk == 0;
-    const int KT = (r1 - r0 + KR - 1) / KR;
-    auto issue = [&](int kt) {
-        char* buf = smem + (kt & 1) * BUF;
-        sy.issue(buf, kt);
-        sx.issue(buf + BN * STAGE_BYTES, kt);
-    };
-    auto commit = [&](int kt) {
-        char* buf = smem + (kt & 1) * BUF;
-        sy.commit(buf);
-        sx.commit(buf + BN * STAGE_BYTES);
-    };
-    if (KT > 0) {
-        sy.fetch(0);
-        sx.fetch(0);
-        issue(0);
-        commit(0);
-    }
-    for (int kt = 0; kt < KT; ++kt) {
-        stage_barrier<DMA>();
-        if (kt + 1 < KT) issue(kt + 1);
-        const char* a = smem + (kt & 1) * BUF;
-        const char* b = a + BN * STAGE_BYTES;
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            u32x4 fa[FN], fb[FK];
-#pragma unroll
-            for (int f = 0; f < FN; ++f) fa[f] = frag_fc<T, BN>(a, wn * (BN / WN) + f * 16, s, lane);
-#pragma unroll
-            for (int j = 0; j < FK; ++j) fb[j] = frag_fc<T, BK>(b, wk * (BK / WK) + j * 16, s, lane);
-#pragma unroll
-            for (int j = 0; j < FK; ++j)
-#pragma unroll
-                for (int f = 0; f < FN; ++f) acc[j][f] = M::mul(fb[j], fa[f], acc[j][f]);
-            if (bias)
-#pragma unroll
-                for (int f = 0; f < FN; ++f) sum[f] = M::mul(M::ones(), fa[f], sum[f]);
-        }
-        if (kt + 1 < KT) commit(kt + 1);
-    }
     const bool whole = p.splits == 1;
     const int64_t nk = (int64_t)p.N * p.K, gnk = p.G * nk;
+    if (tk < 0) {   // a thread takes one chunk of every RL-th row, four rows at a time; the RL sums meet in LDS, in order
+        constexpr int E = CHUNK / (int)sizeof(T), CW = BT / E, RL = NT / CW;
+        float* part = reinterpret_cast<float*>(smem);   // [RL][BT]
+        const int c = tid % CW, rl = tid / CW;
+        const int64_t width = (int64_t)p.N * sizeof(T), byte = ((int64_t)n0 + c * E) * sizeof(T);
+        float s[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) s[e] = 0.0f;
+        for (int r = r0 + rl; r < r1; r += 4 * RL) {
+            u32x4 v[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int row = r + u * RL;
+                int src = min(row, r1 - 1);
+                if (p.m_dy) src = p.list[src];
+                v[u] = u32x4{0, 0, 0, 0};
+                if (row < r1 && src >= 0 && src < p.P) v[u] = load_chunk<T>(p.dy + (int64_t)src * p.lddy, byte, width, (int64_t)(n0 + BT) * (int64_t)sizeof(T) <= width);
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                T t[E];
+                __builtin_memcpy(t, &v[u], CHUNK);
+#pragma unroll
+                for (int e = 0; e < E; ++e) s[e] += (float)t[e];
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < E; ++e) part[rl * BT + c * E + e] = s[e];
+        __syncthreads();
+        for (int i = tid; i < BT; i += NT) {
+            const int n = n0 + i;
+            float sum = part[i];
+            for (int l = 1; l < RL; ++l) sum += part[l * BT + i];
+            if (n < p.N) {
+                if (whole) reinterpret_cast<O*>(p.db)[(int64_t)g * p.N + n] = (O)sum;
+                else p.part[p.splits * gnk + ((int64_t)blockIdx.z * p.G + g) * p.N + n] = sum;
+            }
+        }
+        return;
+    }
+    typename Mma<T>::Acc acc[FK][FN];
+#pragma unroll
+    for (int f = 0; f < FN; ++f)
+#pragma unroll
+        for (int j = 0; j < FK; ++j) acc[j][f] = typename Mma<T>::Acc{};
+    const int KT = (r1 - r0 + KR - 1) / KR;
+    if (KT > 0) {
+        using S = FcStage<T, BT, NT, DMA>;
+        S sy, sx;
+        const int64_t wy = (int64_t)p.N * sizeof(T), wx = (int64_t)p.K * sizeof(T);
+        sy.init((int64_t)n0 * sizeof(T), wy);
+        sx.init((int64_t)k0 * sizeof(T), wx);
+        int at[S::N], next[S::N];   // the pair at this thread's rows of the stage that is issued (negative: none), and what the list holds for the one behind it
+        const auto row_of = [&](int kt, int i) { return r0 + kt * KR + S::k_of(i); };   // of the grouped order
+        const auto pick = [](int mask, int a, int b) { return (a & mask) | (b & ~mask); };   // (masks, not conditions: the loop stays one block)
+        const auto fetch = [&](int kt) {
+#pragma unroll
+            for (int i = 0; i < S::N; ++i) next[i] = p.list[min(row_of(kt, i), r1 - 1) & p.m_list];
+        };
+        const auto before = [&](int kt) {   // fetched a stage ahead; what is fetched now is older than the loads into LDS that follow
+#pragma unroll
+            for (int i = 0; i < S::N; ++i) {
+                const int row = row_of(kt, i), o = pick(p.m_list, next[i], row);
+                at[i] = row < r1 && o < p.P ? o : -1;
+            }
+            fetch(kt + 1);
+        };
+        const auto issue = [&](int kt, int i) {
+            char* buf = smem + (kt & 1) * BUF;
+            const int l = i % S::N;
+            const bool live = at[l] >= 0;
+            if (i < S::N) sy.issue(buf, p.dy + (uint64_t)(unsigned)pick(p.m_dy, at[l], row_of(kt, l)) * p.lddy, live, wy, l);
+            else sx.issue(buf + BT * STAGE_BYTES, p.x + (uint64_t)(unsigned)pick(p.m_x, p.by_copies(at[l]), row_of(kt, l)) * p.ldx, live, wx, l);
+        };
+        const auto commit = [&](int kt) {
+            char* buf = smem + (kt & 1) * BUF;
+            sy.commit(buf);
+            sx.commit(buf + BT * STAGE_BYTES);
+        };
+        fetch(0);
+        tile_loop<T, FK, FN, (FK + FN) * (sizeof(T) == 4 ? 4 : 2), 2 * S::N, DMA>(KT, acc, before, issue, commit,
+            [&](int kt, int st, int i, u32x4 (&fb)[FK], u32x4 (&fa)[FN]) {
+                const char* a = smem + (kt & 1) * BUF;
+                const char* b = a + BT * STAGE_BYTES;
+                if (i < FN) fa[i] = frag_fc<T, BT>(a, wn * (BT / WN) + i * 16, st, lane);
+                else fb[i - FN] = frag_fc<T, BT>(b, wk * (BT / WK) + (i - FN) * 16, st, lane);
+            });
+    }
     char* dst = whole ? p.dw + g * nk * (int64_t)sizeof(O) : reinterpret_cast<char*>(p.part + blockIdx.z * gnk + g * nk);
-    const bool vec = p.K % 4 == 0 && ((uintptr_t)p.dw % (4 * sizeof(O))) == 0;   // (the workspace is 16-byte aligned: checked by the host)
 #pragma unroll
     for (int f = 0; f < FN; ++f) {
-        const int n = n0 + wn * (BN / WN) + f * 16 + (lane & 15);
+        const int n = n0 + wn * (BT / WN) + f * 16 + (lane & 15);
         if (n >= p.N) continue;
 #pragma unroll
         for (int j = 0; j < FK; ++j) {
-            const int k = k0 + wk * (BK / WK) + j * 16 + (lane >> 4) * 4;
+            const int k = k0 + wk * (BT / WK) + j * 16 + (lane >> 4) * 4;
             const float v[4] = {acc[j][f][0], acc[j][f][1], acc[j][f][2], acc[j][f][3]};
-            if (whole) store4<O>(dst + (int64_t)n * p.K * sizeof(O), k, p.K, v, vec);
-            else store4<float>(dst + (int64_t)n * p.K * sizeof(float), k, p.K, v, p.K % 4 == 0);
-        }
-        if (bias && lane < 16) {   // (the product with ones has the same sum in every first index)
-            const float v = sum[f][0];
-            if (whole) reinterpret_cast<O*>(p.db)[(int64_t)g * p.N + n] = (O)v;
-            else p.part[p.splits * gnk + ((int64_t)blockIdx.z * p.G + g) * p.N + n] = v;
+            if (whole) store4<O>(dst + (int64_t)n * p.K * sizeof(O), k, p.K, v, DMA || p.vec);
+            else store4<float>(dst + (int64_t)n * p.K * sizeof(float), k, p.K, v, DMA || p.vec);
         }
     }
 }

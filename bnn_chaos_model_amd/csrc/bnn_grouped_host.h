@@ -14,52 +14,152 @@ namespace bnn {
 template <typename T> struct Tag { using type = T; };
 
 inline int type_size(int dtype) { return dtype == BNN_TYPE_F32 ? 4 : 2; }
+inline bool aligned(int64_t v, int to) { return v % to == 0; }
+inline bool aligned(const void* v, int to) { return (uintptr_t)v % to == 0; }
+inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// row tiles of BM that P grouped rows of G members (and nobody's) can need
+// row tiles of BM that P grouped rows of G members (and nobody's) can need at most
 inline int64_t row_tiles(const RowsParams& p, int BM) {
-    return p.offsets ? p.P / BM + std::min<int64_t>((int64_t)p.G + 1, p.P) : ((int64_t)p.P + BM - 1) / BM;
+    return p.offsets ? p.P / BM + std::min<int64_t>((int64_t)p.G + 1, p.P) : ceil_div(p.P, BM);
+}
+// ... and about how many they will need: every member's last tile is half empty
+inline int64_t likely_tiles(const RowsParams& p, int BM) {
+    const int64_t used = std::min(p.G, p.P);
+    return p.offsets ? std::max<int64_t>(used, p.P / BM + used / 2) : ceil_div(p.P, BM);
+}
+
+inline int set_grid(RowsParams& p, int BM, int BN, int band) {
+    p.tiles_n = (int32_t)ceil_div(p.N, BN);
+    const int64_t nblk = row_tiles(p, BM) * p.tiles_n;
+    if (nblk > 0x7fffffffLL) return fail(BNN_ERR_RANGE, "too many tiles for one launch");
+    p.nblk = (int32_t)nblk;
+    p.band = band;
+    return 0;
 }
 
 template <typename T, typename O, int BM, int BN, int WM, int WN, bool WFC, bool DMA>
 int launch_rows_tile(RowsParams p, hipStream_t st) {
-    p.tiles_n = (p.N + BN - 1) / BN;
-    const int64_t tm = row_tiles(p, BM), nblk = tm * p.tiles_n;
-    if (nblk > 0x7fffffffLL) return fail(BNN_ERR_RANGE, "too many tiles for one launch");
-    p.nblk = (int32_t)nblk;
-    p.band = 8;
+    if (int rc = set_grid(p, BM, BN, 8)) return rc;
     constexpr auto* kern = &bnn_grouped_kernel<T, O, BM, BN, WM, WN, WFC, DMA>;
     allow_big_lds<kern>();
-    hipLaunchKernelGGL(*kern, dim3((unsigned)nblk), dim3(WM * WN * 64), (size_t)2 * (BM + BN) * STAGE_BYTES, st, p);
+    hipLaunchKernelGGL(*kern, dim3((unsigned)p.nblk), dim3(WM * WN * 64), (size_t)2 * (BM + BN) * STAGE_BYTES, st, p);
     HIP_TRY(hipGetLastError());
     return 0;
 }
 
+template <typename T, typename O, int FM, int FN, int U, bool VEC>
+int launch_rows_few(RowsParams p, hipStream_t st) {
+    if (int rc = set_grid(p, 16 * FM, 16 * FN, 1)) return rc;
+    constexpr auto* kern = &bnn_grouped_few_kernel<T, O, FM, FN, U, VEC>;
+    allow_big_lds<kern>();
+    hipLaunchKernelGGL(*kern, dim3((unsigned)p.nblk), dim3(512), (size_t)8 * FM * FN * 64 * 16, st, p);
+    HIP_TRY(hipGetLastError());
+    return 0;
+}
+
+template <typename T, typename O, bool VEC>
+int launch_few(const RowsParams& p, hipStream_t st) {
+    if (likely_tiles(p, 16) > std::min(p.G, p.P)) return launch_rows_few<T, O, 2, 2, 4, VEC>(p, st);        // more than 16 rows a member
+    if (likely_tiles(p, 16) * ceil_div(p.N, 16) <= 512) return launch_rows_few<T, O, 1, 1, 8, VEC>(p, st);   // two workgroups per CU
+    return launch_rows_few<T, O, 1, 2, 4, VEC>(p, st);
+}
+
+template <typename T, typename O, int FN, int ST>
+int launch_rows_short(RowsParams p, hipStream_t st) {
+    // rows per workgroup: as many as let the grid run in whole rounds of two workgroups per CU (320 rows, one round, for 150 000 rows x 128
+    // outputs: 44 us; 256 rows, a fifth more workgroups: 62)
+    const int64_t tiles_n = ceil_div(p.N, 16 * FN), loss = std::min(p.G, p.P) * tiles_n;
+    int64_t room = 512;
+    while (room <= loss) room += 512;
+    p.block_rows = (int32_t)std::max<int64_t>(64, ceil_div(ceil_div(p.P * tiles_n, room - loss / 2), 64) * 64);
+    if (int rc = set_grid(p, p.block_rows, 16 * FN, 1)) return rc;
+    hipLaunchKernelGGL((bnn_grouped_short_kernel<T, O, FN, ST>), dim3((unsigned)p.nblk), dim3(256), 0, st, p);
+    HIP_TRY(hipGetLastError());
+    return 0;
+}
+
+template <typename T, typename O, int ST>
+int launch_short(const RowsParams& p, hipStream_t st) {
+    return p.N <= 64 ? launch_rows_short<T, O, 4, ST>(p, st) : launch_rows_short<T, O, 8, ST>(p, st);
+}
+
+// whole, aligned 16-byte chunks along every staged row (and four aligned outputs per store: p.vec)
+template <typename T>
+bool whole_chunks(const RowsParams& p, bool wfc) {
+    return p.vec && aligned(p.x, CHUNK) && aligned(p.ldx, CHUNK) && aligned((int64_t)p.K * sizeof(T), CHUNK) && aligned(p.w, CHUNK) && aligned(p.w_member, CHUNK) &&
+           aligned(p.w_row, CHUNK) && (!wfc || aligned((int64_t)p.N * sizeof(T), CHUNK));
+}
+
+// Which kernel.  The tiles' costs are rounds of the chip times the measured cost of a round, in units of a 256 x 256 tile (one workgroup per CU;
+// two of 128 x 128, four of 64 x 64): the larger tile reads LDS and L2 less per product, the smaller ones leave fewer CUs and rows idle.
 template <typename T, typename O, bool WFC>
-int launch_rows_typed(const RowsParams& p, hipStream_t st) {
+int launch_rows_typed(RowsParams p, hipStream_t st) {
+    p.vec = p.N % 4 == 0 && aligned(p.ldy, 4 * sizeof(O)) && aligned(p.y, 4 * sizeof(O));
+    const bool dma = whole_chunks<T>(p, WFC);
+    const auto tiles = [&](int BM, int BN) { return likely_tiles(p, BM) * ceil_div(p.N, BN); };
+    const int64_t steps = ceil_div((int64_t)p.K * sizeof(T), 64), used = std::min(p.G, p.P);
+    if constexpr (!WFC) {
+        // few rows a member and not enough 64 x 64 tiles to fill the chip: split the reduction over a workgroup's waves instead
+        // (one row x 4 096 x 4 096 in 8 bits: 5.6 us against 13.2; 480 rows of 30 members, 480 tiles: 26 against 16)
+        if (p.P <= 64 * used && tiles(64, 64) <= 320) return dma ? launch_few<T, O, true>(p, st) : launch_few<T, O, false>(p, st);
+        // rows of up to 256 bytes that cannot be loaded straight into LDS (150 000 x 41 -> 128: 44 us against 61)
+        if (!dma && steps <= 4 && p.P >= 64 * used) {
+            if (steps <= 1) return launch_short<T, O, 1>(p, st);
+            if (steps == 2) return launch_short<T, O, 2>(p, st);
+            return steps == 3 ? launch_short<T, O, 3>(p, st) : launch_short<T, O, 4>(p, st);
+        }
+    }
+    // (exact fp32 products: the matrix pipe is the bound in every tile, the small ones lose less)
+    const double r128 = sizeof(T) == 4 ? 0.52 : 0.64, r64 = sizeof(T) == 4 ? 0.27 : 0.5;
+    const double t256 = (double)ceil_div(tiles(256, 256), 256), t128 = ceil_div(tiles(128, 128), 512) * r128, t64 = ceil_div(tiles(64, 64), 1024) * r64;
+    if (dma) {
+        if (t256 <= t128 && t256 <= t64) return launch_rows_tile<T, O, 256, 256, 2, 4, WFC, true>(p, st);
+        if (t128 <= t64) return launch_rows_tile<T, O, 128, 128, 2, 2, WFC, true>(p, st);
+        return launch_rows_tile<T, O, 64, 64, 2, 2, WFC, true>(p, st);
+    }
+    if constexpr (sizeof(T) == 1)   // 16 384 x 4 095 -> 4 096: 542 us against 842 in 128 x 128 tiles
+        if (ceil_div(tiles(256, 128), 256) * 0.41 <= std::min(t128, t64)) return launch_rows_tile<T, O, 256, 128, 4, 2, WFC, false>(p, st);
+    if (t128 <= t64) return launch_rows_tile<T, O, 128, 128, 2, 2, WFC, false>(p, st);
     return launch_rows_tile<T, O, 64, 64, 2, 2, WFC, false>(p, st);
 }
 
 int launch_rows(int dtype, int out, bool wfc, const RowsParams& p, hipStream_t st);
 
-inline int reduce_splits(const bnn_grouped* q) { return 1; }
+// dW: the tile, and into how many parts the rows of a member are cut (by the sizes alone: the workspace is asked for before the pointers are known)
+struct ReducePlan { int tile, splits; };
+inline ReducePlan reduce_plan(int64_t P, int64_t G, int64_t N, int64_t K, bool f32) {
+    const auto tiles = [&](int b) { return G * ceil_div(N, b) * ceil_div(K, b); };
+    if (!f32 && tiles(256) >= 192) return {256, 1};
+    if (tiles(128) >= 192) return {128, 1};
+    // about two rounds of four workgroups per CU, at least 256 rows each
+    return {64, (int)std::max<int64_t>(1, std::min<int64_t>({2048 / tiles(64), P / G / 256, 16}))};
+}
 
-template <typename T, int BN, int BK, int WN, int WK, bool DMA>
+template <typename T, int BT, int WN, int WK, bool DMA>
 int launch_reduce_tile(ReduceParams p, hipStream_t st) {
-    p.tiles_k = (p.K + BK - 1) / BK;
-    const int64_t tiles = (int64_t)((p.N + BN - 1) / BN) * p.tiles_k;
+    p.tiles_k = (int32_t)ceil_div(p.K, BT);
+    const int64_t tiles = ceil_div(p.N, BT) * (p.tiles_k + (p.db ? 1 : 0));
     if (tiles > 0x7fffffffLL || p.G > 65535) return fail(BNN_ERR_RANGE, "dW takes up to 65535 members");
-    constexpr auto* kern = &bnn_grouped_dw_kernel<T, T, BN, BK, WN, WK, DMA>;
+    constexpr auto* kern = &bnn_grouped_dw_kernel<T, T, BT, WN, WK, DMA>;
     allow_big_lds<kern>();
-    hipLaunchKernelGGL(*kern, dim3((unsigned)tiles, (unsigned)p.G, (unsigned)p.splits), dim3(WN * WK * 64), (size_t)2 * (BN + BK) * STAGE_BYTES, st, p);
+    hipLaunchKernelGGL(*kern, dim3((unsigned)tiles, (unsigned)p.G, (unsigned)p.splits), dim3(WN * WK * 64), (size_t)4 * BT * STAGE_BYTES, st, p);
     HIP_TRY(hipGetLastError());
     return 0;
 }
 
 template <typename T>
-int launch_reduce_typed(const ReduceParams& p, hipStream_t st) {
-    return launch_reduce_tile<T, 64, 64, 2, 2, false>(p, st);
+int launch_reduce_typed(ReduceParams p, int tile, hipStream_t st) {
+    p.vec = p.K % 4 == 0 && aligned(p.dw, 4 * sizeof(T));
+    const bool dma = p.vec && aligned(p.x, CHUNK) && aligned(p.dy, CHUNK) && aligned(p.ldx, CHUNK) && aligned(p.lddy, CHUNK) && aligned((int64_t)p.K * sizeof(T), CHUNK) &&
+                     aligned((int64_t)p.N * sizeof(T), CHUNK);
+    if (dma) {
+        if constexpr (sizeof(T) == 2)
+            if (tile == 256) return launch_reduce_tile<T, 256, 2, 4, true>(p, st);
+        return tile == 128 ? launch_reduce_tile<T, 128, 2, 4, true>(p, st) : launch_reduce_tile<T, 64, 2, 2, true>(p, st);
+    }
+    return tile >= 128 ? launch_reduce_tile<T, 128, 2, 4, false>(p, st) : launch_reduce_tile<T, 64, 2, 2, false>(p, st);
 }
 
-int launch_reduce(int dtype, const ReduceParams& p, hipStream_t st);
+int launch_reduce(int dtype, const ReduceParams& p, int tile, hipStream_t st);
 
 }  // namespace bnn

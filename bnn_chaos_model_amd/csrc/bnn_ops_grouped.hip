@@ -170,12 +170,15 @@ namespace {
 
 unsigned sweep_blocks(int64_t n) { return (unsigned)std::min<int64_t>(std::max<int64_t>((n + 255) / 256, 1), 256 * 16); }
 
+ReducePlan plan_of(const bnn_grouped* q) { return reduce_plan(q->rows * q->copies, q->members, q->outputs, q->inputs, q->dtype == BNN_TYPE_F32); }
+
 int check_grouped(const bnn_grouped* q, bool int8) {
     if (!q) return fail(BNN_ERR_INVALID, "grouped descriptor is NULL");
     if (q->dtype < BNN_TYPE_F32 || q->dtype > BNN_TYPE_F16) return fail(BNN_ERR_INVALID, "dtype must be one of bnn_dtype");
     if (q->rows < 0 || q->copies < 1 || q->members < 1 || q->inputs < 1 || q->outputs < 1) return fail(BNN_ERR_INVALID, "bad rows / copies / members / inputs / outputs");
     if (q->rows > 0x7fffffffLL / q->copies) return fail(BNN_ERR_RANGE, "rows x copies must stay below 2^31");
     if (q->inputs > (1 << 24) || q->outputs > (1 << 24) || q->members > (1 << 24)) return fail(BNN_ERR_RANGE, "members, inputs and outputs must stay below 2^24");
+    if (q->x_row < 0 || q->y_row < 0 || q->x_row > (1 << 28) || q->y_row > (1 << 28)) return fail(BNN_ERR_RANGE, "rows must be less than 2^28 elements apart");
     if ((q->gather || q->scatter) && q->rows && !q->order) return fail(BNN_ERR_INVALID, "gather / scatter need order");
     return 0;
 }
@@ -274,7 +277,7 @@ int bnn_grouped_linear_dx(const bnn_grouped* q, const void* dy, const void* w, v
 
 size_t bnn_grouped_linear_dw_workspace_bytes(const bnn_grouped* q) {
     if (!q || q->rows <= 0 || q->members < 1 || q->inputs < 1 || q->outputs < 1) return 0;
-    const int s = reduce_splits(q);
+    const int s = plan_of(q).splits;
     return s > 1 ? (size_t)s * q->members * q->outputs * ((size_t)q->inputs + 1) * sizeof(float) : 0;
 }
 
@@ -284,13 +287,17 @@ int bnn_grouped_linear_dw(const bnn_grouped* q, const void* dy, const void* x, v
     const int es = type_size(q->dtype);
     ReduceParams p{};
     p.x = (const char*)x; p.dy = (const char*)dy; p.dw = (char*)dw; p.db = db; p.part = (float*)workspace;
-    p.order = q->order; p.offsets = q->offsets;
-    p.ldx = q->x_row * es; p.lddy = q->y_row * es;
+    p.offsets = q->offsets;
+    p.ldx = (uint32_t)(q->x_row * es); p.lddy = (uint32_t)(q->y_row * es);
     p.P = (int32_t)(q->rows * q->copies); p.G = q->members; p.N = q->outputs; p.K = q->inputs;
-    p.x_div = q->gather ? q->copies : 0; p.dy_div = q->scatter ? 1 : 0;
-    p.splits = q->rows ? reduce_splits(q) : 1;
+    p.m_x = q->gather ? -1 : 0; p.m_dy = q->scatter ? -1 : 0; p.m_list = p.m_x | p.m_dy;
+    p.list = p.m_list ? q->order : q->offsets;
+    while ((1LL << p.shift) < q->copies) ++p.shift;   // pair / copies = (2 pair * magic >> 32) >> shift, exact below 2^31: magic = ceil(2^(31 + shift) / copies)
+    p.magic = (uint32_t)(((1ULL << (31 + p.shift)) + q->copies - 1) / q->copies);
+    const ReducePlan plan = plan_of(q);
+    p.splits = q->rows ? plan.splits : 1;
     if (p.splits > 1 && (!workspace || (uintptr_t)workspace % 16)) return fail(BNN_ERR_INVALID, "workspace is NULL or not 16-byte aligned");
-    if (int rc = launch_reduce(q->dtype, p, (hipStream_t)stream)) return rc;
+    if (int rc = launch_reduce(q->dtype, p, plan.tile, (hipStream_t)stream)) return rc;
     if (p.splits == 1) return 0;
     const int64_t n = (int64_t)p.G * p.N * p.K, nb = (int64_t)p.G * p.N;
     const float* part = (const float*)workspace;

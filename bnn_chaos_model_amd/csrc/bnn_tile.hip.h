@@ -64,17 +64,42 @@ template <> struct Mma<int8_t> {
 
 // ---- 16-byte loads of rows with any alignment and any length -------------------------------------------------------------------------
 struct __attribute__((packed, aligned(1))) Bytes16 { u32x4 v; };
+__device__ __forceinline__ u32x4 load_any(const char* at) { return reinterpret_cast<const Bytes16*>(at)->v; }
+
+// Bytes [byte, byte + 16) of a row of nbytes >= 16, zero behind it: the row's last 16 bytes at most, shifted down (no branch: the loads of a
+// thread stay in flight together)
 template <typename T>
-__device__ __forceinline__ u32x4 load_chunk(const char* row, int64_t byte, int64_t nbytes) {   // bytes [byte, byte + 16) of a row of nbytes, zero behind it
-    if (byte + CHUNK <= nbytes) return reinterpret_cast<const Bytes16*>(row + byte)->v;
-    u32x4 r = {0, 0, 0, 0};
-    if (byte >= nbytes) return r;
+__device__ __forceinline__ u32x4 load_tail(const char* row, int64_t byte, int64_t nbytes) {
+    const int64_t at = byte < nbytes - CHUNK ? byte : nbytes - CHUNK;
+    const int d = byte - at < CHUNK ? (int)(byte - at) : CHUNK;
+    u32x4 v = load_any(row + at);
+    if (d & 4) v = u32x4{v.y, v.z, v.w, 0};
+    if (d & 8) v = u32x4{v.z, v.w, 0, 0};
+    if (d & 16) v = u32x4{0, 0, 0, 0};
+    if constexpr (sizeof(T) < 4) {
+        const unsigned s = d & 3;
+        v = u32x4{__builtin_amdgcn_alignbyte(v.y, v.x, s), __builtin_amdgcn_alignbyte(v.z, v.y, s), __builtin_amdgcn_alignbyte(v.w, v.z, s),
+                  __builtin_amdgcn_alignbyte(0, v.w, s)};
+    }
+    return v;
+}
+// the same for rows shorter than that
+template <typename T>
+__device__ __forceinline__ u32x4 load_short(const char* row, int64_t byte, int64_t nbytes) {
+    u32x4 r;
     T tmp[CHUNK / sizeof(T)];
 #pragma unroll
     for (int i = 0; i < (int)(CHUNK / sizeof(T)); ++i)
         tmp[i] = byte + (int64_t)((i + 1) * sizeof(T)) <= nbytes ? reinterpret_cast<const T*>(row + byte)[i] : (T)0;
     __builtin_memcpy(&r, tmp, CHUNK);
     return r;
+}
+// inside: the caller knows (for all lanes) that the chunk ends within the row
+template <typename T>
+__device__ __forceinline__ u32x4 load_chunk(const char* row, int64_t byte, int64_t nbytes, bool inside) {
+    if (inside) return load_any(row + byte);
+    if (nbytes >= CHUNK) return load_tail<T>(row, byte, nbytes);
+    return load_short<T>(row, byte, nbytes);
 }
 
 static __device__ __attribute__((aligned(16))) const uint32_t zero_chunk[4] = {0, 0, 0, 0};   // where a lane outside the reduction reads
@@ -104,6 +129,11 @@ __device__ __forceinline__ u32x4 frag_kc(const char* tile, int row0, int s, int 
     const int row = row0 + (lane & 15);
     return *reinterpret_cast<const u32x4*>(tile + row * STAGE_BYTES + (((s * 4 + (lane >> 4)) ^ kc_swz(row)) << 4));
 }
+// The transposing read of four rows: lanes 4 j .. 4 j + 3 of a group of 16 give row j, lane i receives column i.  (The pointer is restrict: it never
+// meets a load into LDS that is still under way -- the waits are written in the loop -- and without the word the compiler waits for all of them.)
+__device__ __forceinline__ u32x2 read_transposed(const BNN_LDS s16x4* __restrict__ a) {
+    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((BNN_LDS s16x4*)a));
+}
 template <typename T, int W>
 __device__ __forceinline__ u32x4 frag_fc(const char* tile, int col0, int s, int lane) {
     const int q = lane >> 4, i = lane & 15;
@@ -115,14 +145,14 @@ __device__ __forceinline__ u32x4 frag_fc(const char* tile, int col0, int s, int 
             r[j] = *reinterpret_cast<const uint32_t*>(tile + k * W * 4 + (((col >> 2) ^ fc_swz<T, W>(k)) << 4) + (col & 3) * 4);
         }
         return r;
-    } else {   // the transposing read: lanes 4 j .. 4 j + 3 of a group of 16 give row j, lane i receives column i of the four rows
+    } else {
         u32x4 r;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const int k = s * 32 + 8 * q + 4 * h + (i >> 2);
             const int chunk = (col0 >> 3) + ((i & 3) >> 1);
             const char* a = tile + k * W * 2 + ((chunk ^ fc_swz<T, W>(k)) << 4) + (i & 1) * 8;
-            const u32x2 v = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((BNN_LDS s16x4*)a));
+            const u32x2 v = read_transposed((const BNN_LDS s16x4*)a);
             r[2 * h] = v.x;
             r[2 * h + 1] = v.y;
         }
@@ -135,8 +165,7 @@ struct RowTile { int g, r0, r1; };   // member, first row and end of the tile's 
 
 // Tile `t` of the grouped rows cut into pieces of BM per member.  Every wave finds it by itself: a lane takes the member(s) of its index, the
 // tile counts are summed along the wave.  Offsets out of order or out of range are clamped to [0, P]: rows may then be wrong, accesses not.
-template <int BM>
-__device__ __forceinline__ RowTile find_rows(const int32_t* __restrict__ off, int G, int P, int t) {
+__device__ __forceinline__ RowTile find_rows(const int32_t* __restrict__ off, int G, int P, int t, int BM) {
     const int lane = threadIdx.x & 63;
     if (off == nullptr) {
         const int64_t r0 = (int64_t)t * BM;

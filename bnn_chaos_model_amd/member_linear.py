@@ -66,7 +66,7 @@ def _addr(t):
 
 def _rows2d(t):
     """t [n, K] with its elements side by side in a row; rows may be any distance apart (a slice, an expanded row)."""
-    return t if t.shape[1] <= 1 or t.stride(1) == 1 else t.contiguous()
+    return t if (t.shape[1] <= 1 or t.stride(1) == 1) and t.stride(0) <= 1 << 28 else t.contiguous()
 
 
 def _row_stride(t):
