@@ -135,7 +135,9 @@ def lib():
     L.bnn_grouped_linear_dx.argtypes = [G, _vp, _vp, _vp, _vp, _vp]
     L.bnn_grouped_linear_dw_workspace_bytes.argtypes = [G]
     L.bnn_grouped_linear_dw.argtypes = [G, _vp, _vp, _vp, _vp, _vp, _vp]
-    for f in (L.bnn_group_rows_workspace_bytes, L.bnn_grouped_linear_dx_workspace_bytes, L.bnn_grouped_linear_dw_workspace_bytes):
+    L.bnn_int8_linear_rows_workspace_bytes.argtypes = [G]
+    L.bnn_int8_linear_rows.argtypes = [G, _vp, C.c_int32, _vp, _vp, _vp, _vp, _vp, _vp]
+    for f in (L.bnn_group_rows_workspace_bytes, L.bnn_int8_linear_rows_workspace_bytes, L.bnn_grouped_linear_dx_workspace_bytes, L.bnn_grouped_linear_dw_workspace_bytes):
         f.restype = C.c_size_t
     L.bnn_relu_grad.argtypes = [_vp, C.c_int64, _vp, C.c_int64, C.c_int64, C.c_int32, C.c_int32, _vp, _vp]
     L.bnn_quantize_rows.argtypes = [_vp, C.c_int32, C.c_int64, C.c_int32, C.c_int64, _vp, C.c_int64, _vp, _vp]
@@ -153,7 +155,8 @@ EXPORTS = ("bnn_abi_version", "bnn_last_error", "bnn_device_count", "bnn_param_c
            "bnn_sketch_quantiles_f32", "bnn_forward_lowp_f32", "bnn_multiswag_moments_f64", "bnn_multiswag_bands_f32", "bnn_feature_nn_f32", "bnn_spec_source", "bnn_plan_attach_spec",
            "bnn_plan_spec_attached", "bnn_spec_embedded_source", "bnn_gen_params_bytes", "bnn_nonfinite_record_bytes", "bnn_nonfinite_scan_f32",
            "bnn_group_rows_workspace_bytes", "bnn_group_rows_i32", "bnn_grouped_linear", "bnn_grouped_linear_dx_workspace_bytes", "bnn_grouped_linear_dx",
-           "bnn_grouped_linear_dw_workspace_bytes", "bnn_grouped_linear_dw", "bnn_relu_grad", "bnn_quantize_rows", "bnn_int8_linear")
+           "bnn_grouped_linear_dw_workspace_bytes", "bnn_grouped_linear_dw", "bnn_relu_grad", "bnn_quantize_rows", "bnn_int8_linear",
+           "bnn_int8_linear_rows_workspace_bytes", "bnn_int8_linear_rows")
 
 
 def check(rc):

@@ -14,32 +14,41 @@ using namespace bnn;
 // ---- group_rows: a stable counting sort -----------------------------------------------------------------------------------------------------
 // One wave takes 64 consecutive pairs at a time, in order: the lanes that hold the same member are found with one ballot per bit of the key, a
 // lane's place is the number of such lanes before it, and the wave's running count per member lives in LDS.  Pairs of nobody (member outside
-// [0, G)) take key G and come last.  Two sweeps over the keys: counts per (member, block), then places.
-constexpr int GROUP_CHUNK = 8192;      // pairs per workgroup
+// [0, G)) take key G and come last.  Counts per (member, block), their prefix sums, then places; up to GROUP_CHUNK pairs one workgroup does it
+// all.  A thread's keys are loaded at once and stay in registers.
+constexpr int GROUP_CHUNK = 4096;      // pairs per workgroup
 constexpr int GROUP_MAX_MEMBERS = 4096;
 
-__device__ __forceinline__ int key_of(const int32_t* member, int64_t i, int G) {
-    const int m = member[i];
-    return m >= 0 && m < G ? m : G;
-}
-
-// counts of this workgroup's pairs: wc[wave][G + 1]
 template <int WAVES>
-__device__ __forceinline__ void count_chunk(const int32_t* member, int64_t lo, int64_t hi, int G, int32_t* wc) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, G1 = G + 1;
-    for (int i = threadIdx.x; i < WAVES * G1; i += WAVES * 64) wc[i] = 0;
-    __syncthreads();
-    constexpr int per = GROUP_CHUNK / WAVES;
-    const int64_t a = lo + wave * per, e = min(hi, a + per);
-    for (int64_t i = a + lane; i < e; i += 64) atomicAdd(&wc[wave * G1 + key_of(member, i, G)], 1);   // (whole numbers: any order gives the same counts)
-    __syncthreads();
-}
+struct Keys {
+    static constexpr int PER = GROUP_CHUNK / WAVES, N = PER / 64;
+    int key[N];   // of pairs lo + wave * PER + i * 64 + lane; -1 behind the end
+    __device__ __forceinline__ void load(const int32_t* __restrict__ member, int64_t lo, int64_t P, int G) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int64_t at = pair(lo, i);
+            const int m = member[at < P ? at : P - 1];
+            key[i] = at >= P ? -1 : m >= 0 && m < G ? m : G;
+        }
+    }
+    __device__ __forceinline__ int64_t pair(int64_t lo, int i) const { return lo + (int64_t)(threadIdx.x >> 6) * PER + i * 64 + (threadIdx.x & 63); }
+    // this workgroup's counts: wc[wave][G + 1]
+    __device__ __forceinline__ void count(int G, int32_t* wc) const {
+        for (int i = threadIdx.x; i < WAVES * (G + 1); i += WAVES * 64) wc[i] = 0;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (key[i] >= 0) atomicAdd(&wc[(threadIdx.x >> 6) * (G + 1) + key[i]], 1);   // (whole numbers: any order gives the same counts)
+        __syncthreads();
+    }
+};
 
 template <int WAVES>
 __global__ __launch_bounds__(WAVES * 64) void bnn_group_count_kernel(const int32_t* __restrict__ member, int64_t P, int G, int32_t* __restrict__ cnt) {
     extern __shared__ int32_t wc[];
-    const int64_t lo = (int64_t)blockIdx.x * GROUP_CHUNK, hi = min(P, lo + GROUP_CHUNK);
-    count_chunk<WAVES>(member, lo, hi, G, wc);
+    Keys<WAVES> keys;
+    keys.load(member, (int64_t)blockIdx.x * GROUP_CHUNK, P, G);
+    keys.count(G, wc);
     for (int g = threadIdx.x; g <= G; g += WAVES * 64) {
         int32_t s = 0;
         for (int w = 0; w < WAVES; ++w) s += wc[w * (G + 1) + g];
@@ -58,15 +67,35 @@ __device__ __forceinline__ int32_t wave_scan(int32_t v) {
     return v;
 }
 
-// member g's counts over the blocks -> exclusive prefix in place, total behind the table
-__global__ __launch_bounds__(64) void bnn_group_scan_kernel(int32_t* __restrict__ cnt, int nb, int32_t* __restrict__ total) {
+// member g's counts over the blocks -> exclusive prefix in place, total behind the table; 1 024 counts a sweep, four to a thread
+__global__ __launch_bounds__(256) void bnn_group_scan_kernel(int32_t* __restrict__ cnt, int nb, int32_t* __restrict__ total) {
+    __shared__ int32_t wsum[4];
     int32_t* row = cnt + (int64_t)blockIdx.x * nb;
+    const int wave = threadIdx.x >> 6;
     int32_t carry = 0;
-    for (int b0 = 0; b0 < nb; b0 += 64) {
-        const int b = b0 + threadIdx.x;
-        const int32_t v = b < nb ? row[b] : 0, inc = wave_scan(v);
-        if (b < nb) row[b] = carry + inc - v;
-        carry += __shfl(inc, 63);
+    for (int b0 = 0; b0 < nb; b0 += 1024) {
+        int32_t v[4], sum = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int b = b0 + threadIdx.x * 4 + i;
+            v[i] = b < nb ? row[b] : 0;
+            sum += v[i];
+        }
+        const int32_t inc = wave_scan(sum);
+        if ((threadIdx.x & 63) == 63) wsum[wave] = inc;
+        __syncthreads();
+        int32_t at = carry + inc - sum;
+        for (int w = 0; w < 4; ++w) {
+            if (w < wave) at += wsum[w];
+            carry += wsum[w];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int b = b0 + threadIdx.x * 4 + i;
+            if (b < nb) row[b] = at;
+            at += v[i];
+        }
     }
     if (threadIdx.x == 0) total[blockIdx.x] = carry;
 }
@@ -79,15 +108,22 @@ __global__ __launch_bounds__(WAVES * 64) void bnn_group_place_kernel(const int32
     extern __shared__ int32_t wc[];   // [WAVES][G + 1] counts -> places, then [G + 1] member starts
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, G1 = G + 1;
     int32_t* start = wc + WAVES * G1;
-    const int64_t lo = (int64_t)blockIdx.x * GROUP_CHUNK, hi = min(P, lo + GROUP_CHUNK);
-    count_chunk<WAVES>(member, lo, hi, G, wc);
-    for (int g = threadIdx.x; g < G1; g += WAVES * 64) {
-        int32_t s = 0;
-        if constexpr (SINGLE) for (int w = 0; w < WAVES; ++w) s += wc[w * G1 + g];
-        else s = total[g];
-        start[g] = s;
+    const int64_t lo = (int64_t)blockIdx.x * GROUP_CHUNK;
+    Keys<WAVES> keys;
+    if (!SINGLE || P > 0) keys.load(member, lo, P, G);
+    else
+        for (int i = 0; i < keys.N; ++i) keys.key[i] = -1;
+    if constexpr (!SINGLE)
+        for (int g = threadIdx.x; g < G1; g += WAVES * 64) start[g] = total[g];
+    keys.count(G, wc);
+    if constexpr (SINGLE) {
+        for (int g = threadIdx.x; g < G1; g += WAVES * 64) {
+            int32_t s = 0;
+            for (int w = 0; w < WAVES; ++w) s += wc[w * G1 + g];
+            start[g] = s;
+        }
+        __syncthreads();
     }
-    __syncthreads();
     if (wave == 0) {
         int32_t carry = 0;
         for (int g0 = 0; g0 < G1; g0 += 64) {
@@ -111,12 +147,10 @@ __global__ __launch_bounds__(WAVES * 64) void bnn_group_place_kernel(const int32
         }
     }
     __syncthreads();
-    constexpr int per = GROUP_CHUNK / WAVES;
-    const int64_t a = lo + wave * per, e = min(hi, a + per);
-    for (int64_t i0 = a; i0 < e; i0 += 64) {   // (uniform per wave)
-        const int64_t i = i0 + lane;
-        const bool in = i < e;
-        const int key = in ? key_of(member, i, G) : 0;
+#pragma unroll
+    for (int i = 0; i < keys.N; ++i) {
+        const int key = keys.key[i];
+        const bool in = key >= 0;
         uint64_t same = __ballot(in);
         for (int b = 0; b < nbits; ++b) {
             const uint64_t set = __ballot(in && ((key >> b) & 1));
@@ -125,7 +159,7 @@ __global__ __launch_bounds__(WAVES * 64) void bnn_group_place_kernel(const int32
         if (in) {
             const int before = __popcll(same & ((1ull << lane) - 1));
             const int32_t at = wc[wave * G1 + key];
-            order[at + before] = (int32_t)i;
+            order[at + before] = (int32_t)keys.pair(lo, i);
             if (before == 0) wc[wave * G1 + key] = at + __popcll(same);   // (every lane of the wave has read `at`: one wave runs in step)
         }
         __builtin_amdgcn_wave_barrier();
@@ -220,7 +254,7 @@ int bnn_group_rows_i32(const int32_t* member, int64_t pairs, int32_t members, in
         allow_big_lds<bnn_group_place_kernel<WAVES, false>>();
         hipLaunchKernelGGL(bnn_group_count_kernel<WAVES>, dim3((unsigned)nb), dim3(WAVES * 64), lds_count, st, member, pairs, members, cnt);
         HIP_TRY(hipGetLastError());
-        hipLaunchKernelGGL(bnn_group_scan_kernel, dim3((unsigned)members + 1), dim3(64), 0, st, cnt, (int)nb, total);
+        hipLaunchKernelGGL(bnn_group_scan_kernel, dim3((unsigned)members + 1), dim3(256), 0, st, cnt, (int)nb, total);
         HIP_TRY(hipGetLastError());
         hipLaunchKernelGGL((bnn_group_place_kernel<WAVES, false>), dim3((unsigned)nb), dim3(WAVES * 64), lds, st, member, pairs, members, (const int32_t*)cnt,
                            (const int32_t*)total, nbits, order, offsets);

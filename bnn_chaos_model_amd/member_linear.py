@@ -30,34 +30,18 @@ def _gpu(t, name, dtypes):
     return t
 
 
-def _same_device(x, **tensors):
-    for name, t in tensors.items():
-        if t is not None and t.device != x.device:
-            raise ValueError(f"{name} is on {t.device}, the rows are on {x.device}")
+def _same_device(dev, name, t):
+    if t.get_device() != dev:
+        raise ValueError(f"{name} is on {t.device}, the rows are on cuda:{dev}")
 
 
-class _on:
-    """The operands' device current for the calls inside (one process may drive several)."""
-    __slots__ = ("ctx",)
-
-    def __init__(self, t):
-        self.ctx = None if t.device.index == N.current_device() else torch.cuda.device(t.device)
-
-    def __enter__(self):
-        if self.ctx is not None:
-            self.ctx.__enter__()
-
-    def __exit__(self, *exc):
-        if self.ctx is not None:
-            self.ctx.__exit__(*exc)
-
-
-def _stream(t):
-    return N.stream_ptr(t.device.index)
-
-
-def _workspace(nbytes, t):
-    return torch.empty(nbytes, dtype=torch.uint8, device=t.device) if nbytes else None
+def _run(dev, fn, *args):
+    """A native call with device `dev` current (one process may drive several), on torch's current stream of it."""
+    if dev == N.current_device():
+        N.check(fn(*args, N.stream_ptr(dev)))
+    else:
+        with torch.cuda.device(dev):
+            N.check(fn(*args, N.stream_ptr(dev)))
 
 
 def _addr(t):
@@ -66,7 +50,8 @@ def _addr(t):
 
 def _rows2d(t):
     """t [n, K] with its elements side by side in a row; rows may be any distance apart (a slice, an expanded row)."""
-    return t if (t.shape[1] <= 1 or t.stride(1) == 1) and t.stride(0) <= 1 << 28 else t.contiguous()
+    row, col = t.stride()
+    return t if (col == 1 or t.shape[1] <= 1) and row <= 1 << 28 else t.contiguous()
 
 
 def _row_stride(t):
@@ -82,7 +67,7 @@ def group_rows(member, n_members):
     """Sort (row, copy) pairs by ensemble member, stably -> RowGroups(order, offsets, shape).
 
     member: int32 [rows] or [rows, copies], the member(s) that evaluate each row; values outside [0, n_members) mean nobody (padding): those
-    pairs come last, and the layers below give them zeros.  n_members <= 4096.  One launch up to 8192 pairs, three beyond."""
+    pairs come last, and the layers below give them zeros.  n_members <= 4096.  One launch up to 4096 pairs, three beyond."""
     _gpu(member, "member", (torch.int32,))
     if member.dim() not in (1, 2):
         raise ValueError("member must be [rows] or [rows, copies]")
@@ -95,11 +80,11 @@ def group_rows(member, n_members):
     if P >= 2 ** 31:
         raise ValueError("rows x copies must stay below 2^31")
     m = member.contiguous()
-    order = torch.empty((P,), dtype=torch.int32, device=m.device)
-    offsets = torch.empty((n_members + 1,), dtype=torch.int32, device=m.device)
-    with _on(m):
-        ws = _workspace(N.lib().bnn_group_rows_workspace_bytes(P, n_members), m)
-        N.check(N.lib().bnn_group_rows_i32(_addr(m), P, n_members, _addr(order), _addr(offsets), _addr(ws), _stream(m)))
+    order = m.new_empty(P)
+    offsets = m.new_empty(n_members + 1)
+    nbytes = 0 if P <= 4096 else N.lib().bnn_group_rows_workspace_bytes(P, n_members)
+    ws = m.new_empty(nbytes // 4) if nbytes else None
+    _run(m.get_device(), N.lib().bnn_group_rows_i32, m.data_ptr(), P, n_members, order.data_ptr(), offsets.data_ptr(), _addr(ws))
     return RowGroups(order, offsets, tuple(member.shape))
 
 
@@ -110,7 +95,9 @@ def _check_groups(groups, x, G, gather, what="x"):
     order, offsets, shape = groups
     _gpu(order, "groups.order", (torch.int32,))
     _gpu(offsets, "groups.offsets", (torch.int32,))
-    _same_device(x, **{"groups.order": order, "groups.offsets": offsets})
+    dev = x.get_device()
+    _same_device(dev, "groups.order", order)
+    _same_device(dev, "groups.offsets", offsets)
     rows, copies = shape if len(shape) == 2 else (shape[0], 1)
     if order.numel() != rows * copies or not order.is_contiguous() or not offsets.is_contiguous():
         raise ValueError("groups.order must be contiguous and hold one entry per (row, copy) pair")
@@ -138,7 +125,8 @@ def _check_linear(x, weight, groups, bias, gather):
         _gpu(bias, "bias", (x.dtype,))
         if tuple(bias.shape) != (G, n_out):
             raise ValueError(f"bias must be [{G}, {n_out}]")
-    _same_device(x, weight=weight, bias=bias)
+        _same_device(x.get_device(), "bias", bias)
+    _same_device(x.get_device(), "weight", weight)
     return _check_groups(groups, x, G, gather)
 
 
@@ -151,10 +139,9 @@ def _descriptor(groups, rows, copies, dtype, weight, x_row, y_row, gather, scatt
 def _linear(x, weight, groups, bias, relu, gather, scatter, rows, copies):
     x, weight = _rows2d(x), _layers(weight)
     bias = None if bias is None else bias.contiguous()
-    y = torch.empty(_out_shape(groups, weight.shape[1], scatter), dtype=x.dtype, device=x.device)
+    y = x.new_empty(_out_shape(groups, weight.shape[1], scatter))
     q = _descriptor(groups, rows, copies, x.dtype, weight, _row_stride(x), weight.shape[1], gather, scatter, relu)
-    with _on(x):
-        N.check(N.lib().bnn_grouped_linear(C.byref(q), _addr(x), _addr(weight), _addr(bias), _addr(y), _stream(x)))
+    _run(x.get_device(), N.lib().bnn_grouped_linear, q, x.data_ptr(), weight.data_ptr(), _addr(bias), y.data_ptr())
     return y
 
 
@@ -167,35 +154,35 @@ def grouped_linear_grads(dy, x, weight, groups, y=None, gather=False, scatter=Fa
     rows, copies = _check_linear(x, weight, groups, None, gather)
     G, n_out, n_in = weight.shape
     shape = _out_shape(groups, n_out, scatter)
-    _gpu(dy, "dy", (x.dtype,))
-    if tuple(dy.shape) != shape:
-        raise ValueError(f"dy must be {list(shape)}")
-    _same_device(x, dy=dy, y=y)
+    dev = x.get_device()
+    for name, t in (("dy", dy),) if y is None else (("dy", dy), ("y", y)):
+        _gpu(t, name, (x.dtype,))
+        if tuple(t.shape) != shape:
+            raise ValueError(f"{name} must be {list(shape)}")
+        _same_device(dev, name, t)
     x, weight = _rows2d(x), _layers(weight)
     dy = _rows2d(dy.reshape(-1, n_out))
     need_x, need_w, need_b = need
-    with _on(x):
-        L, st = N.lib(), _stream(x)
-        if y is not None:
-            _gpu(y, "y", (x.dtype,))
-            if tuple(y.shape) != shape:
-                raise ValueError(f"y must be {list(shape)}")
-            y2 = _rows2d(y.reshape(-1, n_out))
-            masked = torch.empty((dy.shape[0], n_out), dtype=x.dtype, device=x.device)
-            N.check(L.bnn_relu_grad(_addr(dy), _row_stride(dy), _addr(y2), _row_stride(y2), dy.shape[0], n_out, _TYPES[x.dtype], _addr(masked), st))
-            dy = masked
-        dx = dw = db = None
-        if need_x:
-            dx = torch.empty((x.shape[0], n_in), dtype=x.dtype, device=x.device)
-            q = _descriptor(groups, rows, copies, x.dtype, weight, n_in, _row_stride(dy), gather, scatter)
-            ws = _workspace(L.bnn_grouped_linear_dx_workspace_bytes(C.byref(q)), x)
-            N.check(L.bnn_grouped_linear_dx(C.byref(q), _addr(dy), _addr(weight), _addr(dx), _addr(ws), st))
-        if need_w or need_b:
-            dw = torch.empty((G, n_out, n_in), dtype=x.dtype, device=x.device)
-            db = torch.empty((G, n_out), dtype=x.dtype, device=x.device) if need_b else None
-            q = _descriptor(groups, rows, copies, x.dtype, weight, _row_stride(x), _row_stride(dy), gather, scatter)
-            ws = _workspace(L.bnn_grouped_linear_dw_workspace_bytes(C.byref(q)), x)
-            N.check(L.bnn_grouped_linear_dw(C.byref(q), _addr(dy), _addr(x), _addr(dw), _addr(db), _addr(ws), st))
+    L = N.lib()
+    if y is not None:
+        y2 = _rows2d(y.reshape(-1, n_out))
+        masked = x.new_empty((dy.shape[0], n_out))
+        _run(dev, L.bnn_relu_grad, dy.data_ptr(), _row_stride(dy), y2.data_ptr(), _row_stride(y2), dy.shape[0], n_out, _TYPES[x.dtype], masked.data_ptr())
+        dy = masked
+    dx = dw = db = None
+    if need_x:
+        dx = x.new_empty((x.shape[0], n_in))
+        q = _descriptor(groups, rows, copies, x.dtype, weight, n_in, _row_stride(dy), gather, scatter)
+        nbytes = L.bnn_grouped_linear_dx_workspace_bytes(q)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
+        _run(dev, L.bnn_grouped_linear_dx, q, dy.data_ptr(), weight.data_ptr(), dx.data_ptr(), _addr(ws))
+    if need_w or need_b:
+        dw = x.new_empty((G, n_out, n_in))
+        db = x.new_empty((G, n_out)) if need_b else None
+        q = _descriptor(groups, rows, copies, x.dtype, weight, _row_stride(x), _row_stride(dy), gather, scatter)
+        nbytes = L.bnn_grouped_linear_dw_workspace_bytes(q)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
+        _run(dev, L.bnn_grouped_linear_dw, q, dy.data_ptr(), x.data_ptr(), dw.data_ptr(), _addr(db), _addr(ws))
     return dx, dw if need_w else None, db
 
 
@@ -231,18 +218,6 @@ def grouped_linear(x, weight, groups, bias=None, relu=False, gather=False, scatt
     return _linear(x, weight, groups, bias, relu, gather, scatter, rows, copies)
 
 
-def _quantize(x, pad):
-    K = x.shape[-1]
-    x2 = _rows2d(x.reshape(-1, K))
-    rows = x2.shape[0]
-    ld = (K + pad - 1) // pad * pad
-    q = torch.empty((rows, ld), dtype=torch.int8, device=x.device)
-    scale = torch.empty((rows,), dtype=torch.float32, device=x.device)
-    with _on(x):
-        N.check(N.lib().bnn_quantize_rows(_addr(x2), _TYPES[x.dtype], rows, K, _row_stride(x2), _addr(q), ld, _addr(scale), _stream(x)))
-    return q, scale
-
-
 def _check_quantize(x):
     _gpu(x, "x", tuple(_TYPES))
     if x.dim() < 1 or x.shape[-1] < 1:
@@ -258,8 +233,12 @@ def quantize_rows(x):
     channel of a weight [N, K] / [members, N, K]), values = x / scale rounded half to even, exactly.  A row of zeros has scale 0; a row that holds
     NaN or an infinity has scale NaN, so that whatever is computed from it is NaN."""
     _check_quantize(x)
-    q, scale = _quantize(x, 1)
-    return QuantRows(q.view(x.shape), scale.view(x.shape[:-1]))
+    K = x.shape[-1]
+    x2 = _rows2d(x if x.dim() == 2 else x.reshape(-1, K))
+    values = x.new_empty(x.shape, dtype=torch.int8)
+    scale = x.new_empty(x.shape[:-1], dtype=torch.float32)
+    _run(x.get_device(), N.lib().bnn_quantize_rows, x2.data_ptr(), _TYPES[x.dtype], x2.shape[0], K, _row_stride(x2), values.data_ptr(), K, scale.data_ptr())
+    return QuantRows(values, scale)
 
 
 def int8_linear(x, weight, groups=None, bias=None, relu=False, gather=False, scatter=False, dtype=None):
@@ -297,7 +276,9 @@ def int8_linear(x, weight, groups=None, bias=None, relu=False, gather=False, sca
         if torch.is_grad_enabled() and bias.requires_grad:
             raise NotImplementedError("the 8-bit layer has no gradient: detach bias")
         bias = bias.contiguous()
-    _same_device(rows_of, weight=wq, bias=bias, **{"weight.scale": ws}, **({"x.scale": xs} if quant else {}))
+    dev = rows_of.get_device()
+    for name, t in (("weight.values", wq), ("weight.scale", ws)) + ((("bias", bias),) if bias is not None else ()) + ((("x.scale", xs),) if quant else ()):
+        _same_device(dev, name, t)
     if groups is None:
         if gather or scatter:
             raise ValueError("gather / scatter need groups")
@@ -308,16 +289,17 @@ def int8_linear(x, weight, groups=None, bias=None, relu=False, gather=False, sca
     else:
         rows, copies = _check_groups(groups, rows_of, wq.shape[0], gather)
         shape = _out_shape(groups, wq.shape[1], scatter)
-    if quant:
-        xq, xs = _rows2d(xq), xs.contiguous()
-    else:
-        xq, xs = _quantize(x, 16)   # (rows of whole 16-byte chunks)
+    rows_of = _rows2d(rows_of)
     wq, ws = _layers(wq), ws.contiguous()
-    y = torch.empty(shape, dtype=dtype, device=xq.device)
+    y = rows_of.new_empty(shape, dtype=dtype)
     G, n_out, n_in = wq.shape
-    q = N.BnnGrouped(rows, copies, G, n_in, n_out, _TYPES[dtype], int(bool(gather)), int(bool(scatter)), int(bool(relu)), _row_stride(xq), n_out,
+    q = N.BnnGrouped(rows, copies, G, n_in, n_out, _TYPES[dtype], int(bool(gather)), int(bool(scatter)), int(bool(relu)), _row_stride(rows_of), n_out,
                      wq.stride(0) if G > 1 else 0, wq.stride(1) if n_out > 1 else n_in, None if groups is None else _addr(groups.order),
                      None if groups is None else _addr(groups.offsets))
-    with _on(xq):
-        N.check(N.lib().bnn_int8_linear(C.byref(q), _addr(xq), _addr(xs), _addr(wq), _addr(ws), _addr(bias), _addr(y), _stream(xq)))
+    if quant:
+        xs = xs.contiguous()
+        _run(dev, N.lib().bnn_int8_linear, q, rows_of.data_ptr(), xs.data_ptr(), wq.data_ptr(), ws.data_ptr(), _addr(bias), y.data_ptr())
+    else:
+        space = rows_of.new_empty(max(N.lib().bnn_int8_linear_rows_workspace_bytes(q), 1), dtype=torch.uint8)   # of the codes
+        _run(dev, N.lib().bnn_int8_linear_rows, q, rows_of.data_ptr(), _TYPES[rows_of.dtype], space.data_ptr(), wq.data_ptr(), ws.data_ptr(), _addr(bias), y.data_ptr())
     return y

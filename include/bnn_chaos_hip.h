@@ -397,6 +397,10 @@ int bnn_relu_grad(const void* dy, int64_t dy_row, const void* y, int64_t y_row, 
 int bnn_quantize_rows(const void* x, int32_t dtype, int64_t rows, int32_t K, int64_t x_row, int8_t* q, int64_t q_row, float* scale, void* stream);
 int bnn_int8_linear(const bnn_grouped* q, const int8_t* x, const float* x_scale, const int8_t* w, const float* w_scale, const void* bias, void* y,
                     void* stream);
+/* the same on float rows (x_dtype), quantised on the way as bnn_quantize_rows does; the workspace holds the codes */
+size_t bnn_int8_linear_rows_workspace_bytes(const bnn_grouped* q);
+int bnn_int8_linear_rows(const bnn_grouped* q, const void* x, int32_t x_dtype, void* workspace, const int8_t* w, const float* w_scale, const void* bias, void* y,
+                         void* stream);
 
 /* Raw Philox4x32-10 blocks for known-answer tests: out[n][4] = philox(ctr = {c0+i, c1, c2, c3}, key). */
 int bnn_philox_raw_u32(uint32_t c0, uint32_t c1, uint32_t c2, uint32_t c3, uint32_t k0, uint32_t k1, int64_t n,

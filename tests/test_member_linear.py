@@ -67,7 +67,7 @@ def plain(x, w, b, xi, yi, mem, rows_out):
 
 
 # ---- group_rows --------------------------------------------------------------------------------------------------------------------------
-@pytest.mark.parametrize("n,G,copies", [(0, 3, 0), (1, 1, 0), (1, 30, 0), (63, 30, 0), (64, 2, 2), (65, 7, 3), (8192, 30, 0), (8193, 30, 0), (50001, 1023, 0),
+@pytest.mark.parametrize("n,G,copies", [(0, 3, 0), (1, 1, 0), (1, 30, 0), (63, 30, 0), (64, 2, 2), (65, 7, 3), (4096, 30, 0), (4097, 30, 0), (8192, 30, 0), (8193, 30, 0), (50001, 1023, 0),
                                         (50001, 1024, 2), (20000, 4096, 0), (300007, 30, 4), (1000000, 1, 0)])
 def test_group_rows_is_the_stable_sort(ops, n, G, copies):
     m = members(n, G, copies, seed=n)
@@ -271,7 +271,7 @@ def divide_127(amax):
 
 
 @pytest.mark.parametrize("dtype", list(DT))
-@pytest.mark.parametrize("n,K", [(1, 1), (1, 4096), (15, 41), (64, 40), (1000, 257), (33, 5000), (3, 20001), (2500, 128), (7, 16)])
+@pytest.mark.parametrize("n,K", [(1, 1), (1, 4096), (15, 41), (64, 40), (1000, 257), (33, 5000), (3, 20001), (2500, 128), (2100, 41), (2100, 511), (2100, 1030), (7, 16), (5000, 3)])
 def test_quantize_rows_is_exact(ops, n, K, dtype):
     x = torch.randn(n, K, generator=_gen(K), device="cuda").to(DT[dtype])
     q, s = ops.quantize_rows(x)
@@ -328,7 +328,7 @@ INT8_SLACK = 4 * 2.0 ** -24   # the sum to fp32, the product of the scales, thei
 
 
 @pytest.mark.parametrize("out", list(DT))
-@pytest.mark.parametrize("n,K,N", [(1, 1, 1), (1, 4096, 512), (1, 41, 40), (5, 128, 130), (16, 1040, 64), (17, 4096, 96), (64, 64, 64), (129, 257, 255), (3000, 640, 384), (300, 4099, 16)])
+@pytest.mark.parametrize("n,K,N", [(1, 1, 1), (2, 100, 33), (3, 4096, 64), (4, 15, 16), (9, 4095, 40), (33, 512, 64), (1, 70000, 24), (1, 4096, 512), (1, 41, 40), (5, 128, 130), (16, 1040, 64), (17, 4096, 96), (64, 64, 64), (129, 257, 255), (3000, 640, 384), (300, 4099, 16)])
 def test_int8_linear_dense(ops, n, K, N, out):
     g = _gen(n + K)
     x = (torch.randn(n, K, generator=g, device="cuda") * 3).to(DT[out])
