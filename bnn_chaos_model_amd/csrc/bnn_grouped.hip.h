@@ -30,10 +30,10 @@ struct ReduceParams {          // dW[g] = sum over rows r of member g of dy_r x_
     void* db;                  // [G, N] or null
     float* part;               // [splits, G, N, K] then [splits, G, N] when splits > 1
     const int32_t* offsets;
-    const int32_t* list;       // order if either operand is gathered, else offsets (read, not used)
+    const int32_t* list;       // order, if either operand is gathered
     uint32_t ldx, lddy;
     int32_t P, G, N, K;
-    int32_t m_x, m_dy, m_list;     // -1: row r of the grouped order is row order[r] / copies of x, row order[r] of dy, list is order; 0: row r
+    int32_t m_x, m_dy;             // -1: row r of the grouped order is row order[r] / copies of x, row order[r] of dy; 0: row r
     uint32_t magic, shift;         // of the division by copies
     int32_t tiles_k, splits;
     int32_t vec;                   // K % 4 == 0 and dw aligned to four elements
@@ -69,7 +69,7 @@ template <typename T, int W, int NT, bool DMA>
 struct FcStage {
     static constexpr int CW = W * (int)sizeof(T) / CHUNK, N = W * 8 / NT, KR = stage_k<T>(), STEP = NT / CW;
     static_assert(W * 8 % NT == 0 && NT % CW == 0 && STEP % 8 == 0, "whole chunks per thread, at most two chunk columns per thread");
-    int64_t at[2];     // byte of this thread's chunk in a row: of its even and odd loads
+    int at[2];         // byte of this thread's chunk in a row (below 2^26): of its even and odd loads
     bool inside;       // all of the tile's columns are the matrix's
     u32x4 r[DMA ? 1 : N];
     __device__ __forceinline__ static int k_of(int i) { return threadIdx.x / CW + i * STEP; }
@@ -77,12 +77,12 @@ struct FcStage {
         inside = col0 + W * (int64_t)sizeof(T) <= width;
 #pragma unroll
         for (int o = 0; o < 2; ++o) {
-            at[o] = col0 + (((int)threadIdx.x % CW) ^ fc_swz<T, W>(k_of(o))) * CHUNK;
+            at[o] = (int)col0 + (((int)threadIdx.x % CW) ^ fc_swz<T, W>(k_of(o))) * CHUNK;
             if (DMA && at[o] >= width) at[o] = 0;   // (columns behind the matrix: any, they are not stored)
         }
     }
     __device__ __forceinline__ void issue(char* lds, const char* row, bool live, int64_t width, int i) {   // the i-th of its N loads
-        const int64_t a = at[STEP % 16 == 0 ? 0 : i & 1];
+        const int a = at[STEP % 16 == 0 ? 0 : i & 1];
         if constexpr (DMA) {
             const char* src = row + a;
             load_to_lds(live ? src : (const char*)zero_chunk, lds + (__builtin_amdgcn_readfirstlane(threadIdx.x & ~63) + i * NT) * CHUNK);
@@ -206,14 +206,9 @@ __device__ __forceinline__ void store4(char* row, int n, int N, const float v[4]
 // ---- forward / dX --------------------------------------------------------------------------------------------------------------------------
 // BM rows x BN outputs per workgroup, WM x WN waves.  WFC: the matrix is used the other way round (element (k, n) at k * w_row + n): dX.
 template <typename T, typename O, int BM, int BN, int WM, int WN, bool WFC, bool DMA>
-__global__ __launch_bounds__(WM * WN * 64, WM * WN * 64 >= 512 ? 2 : 1) void bnn_grouped_kernel(RowsParams p) {
+__device__ __forceinline__ void grouped_tile(const RowsParams& p, const RowTile rt, const int tn, char* smem) {
     constexpr int NT = WM * WN * 64, FM = BM / WM / 16, FN = BN / WN / 16, BUF = (BM + BN) * STAGE_BYTES;
     using M = Mma<T>;
-    extern __shared__ __attribute__((aligned(1024))) char smem[];
-    int tm, tn;
-    tile_of_block(p.nblk, p.tiles_n, p.band, tm, tn);
-    const RowTile rt = find_rows(p.offsets, p.G, p.P, tm, BM);
-    if (rt.g < 0) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave / WN, wn = wave % WN;
     const int n0 = tn * BN;
     auto out_row = [&](int m) -> char* {
@@ -327,6 +322,18 @@ __global__ __launch_bounds__(WM * WN * 64, WM * WN * 64 >= 512 ? 2 : 1) void bnn
             store4<O>(row, n0 + wn * (BN / WN) + j * 16 + (lane >> 4) * 4, p.N, v, DMA || p.vec);
         }
     }
+}
+
+template <typename T, typename O, int BM, int BN, int WM, int WN, bool WFC, bool DMA>
+__global__ __launch_bounds__(WM * WN * 64, WM * WN * 64 >= 512 ? 2 : 1) void bnn_grouped_kernel(RowsParams p) {
+    extern __shared__ __attribute__((aligned(1024))) char smem[];
+    int tm, tn;
+    tile_of_block(p.nblk, p.tiles_n, p.band, tm, tn);
+    const RowTile rt = find_rows(p.offsets, p.G, p.P, tm, BM);
+    if (rt.g < 0) return;
+    // a member's last tile: half the rows take half the products (16 members of about 2 048 rows: one tile in nine)
+    if (BM == 256 && rt.r1 - rt.r0 <= BM / 2) grouped_tile<T, O, BM == 256 ? BM / 2 : BM, BN, WM, WN, WFC, DMA>(p, rt, tn, smem);
+    else grouped_tile<T, O, BM, BN, WM, WN, WFC, DMA>(p, rt, tn, smem);
 }
 
 // ---- forward of few rows --------------------------------------------------------------------------------------------------------------------
@@ -517,7 +524,8 @@ __global__ __launch_bounds__(256) void bnn_grouped_short_kernel(RowsParams p) {
 // ---- dW, db --------------------------------------------------------------------------------------------------------------------------------
 // BT outputs x BT inputs of one member per workgroup (blockIdx.y), over split blockIdx.z of the member's rows.  The workgroups in front of the first
 // input tile sum dy's columns (the bias gradient) instead.
-template <typename T, typename O, int BT, int WN, int WK, bool DMA>
+// LISTED: rows of x or dy are found through the order (else both are in grouped order, and a load's row is the wave's plus a constant).
+template <typename T, typename O, int BT, int WN, int WK, bool DMA, bool LISTED>
 __global__ __launch_bounds__(WN * WK * 64, WN * WK * 64 >= 512 ? 2 : 1) void bnn_grouped_dw_kernel(ReduceParams p) {
     constexpr int NT = WN * WK * 64, FN = BT / WN / 16, FK = BT / WK / 16, BUF = 2 * BT * STAGE_BYTES, KR = stage_k<T>();
     extern __shared__ __attribute__((aligned(1024))) char smem[];
@@ -591,19 +599,35 @@ __global__ __launch_bounds__(WN * WK * 64, WN * WK * 64 >= 512 ? 2 : 1) void bnn
         const auto pick = [](int mask, int a, int b) { return (a & mask) | (b & ~mask); };   // (masks, not conditions: the loop stays one block)
         const auto fetch = [&](int kt) {
 #pragma unroll
-            for (int i = 0; i < S::N; ++i) next[i] = p.list[min(row_of(kt, i), r1 - 1) & p.m_list];
+            for (int i = 0; i < S::N; ++i) next[i] = p.list[min(row_of(kt, i), r1 - 1)];
         };
         const auto before = [&](int kt) {   // fetched a stage ahead; what is fetched now is older than the loads into LDS that follow
+            if constexpr (!LISTED) return;
 #pragma unroll
             for (int i = 0; i < S::N; ++i) {
-                const int row = row_of(kt, i), o = pick(p.m_list, next[i], row);
-                at[i] = row < r1 && o < p.P ? o : -1;
+                const int o = next[i];
+                at[i] = row_of(kt, i) < r1 && o < p.P ? o : -1;
             }
             fetch(kt + 1);
         };
+        const char* ly = p.dy + (uint64_t)(unsigned)(r0 + S::k_of(0)) * p.lddy;   // not LISTED: this thread's first rows
+        const char* lx = p.x + (uint64_t)(unsigned)(r0 + S::k_of(0)) * p.ldx;
+        if constexpr (!LISTED && DMA && S::STEP % 16 == 0) {   // ... and its chunk of them (fewer registers in the loop)
+            ly += sy.at[0];
+            lx += sx.at[0];
+            sy.at[0] = sx.at[0] = 0;
+        }
+        const int below = r1 - r0 - S::k_of(0);
         const auto issue = [&](int kt, int i) {
             char* buf = smem + (kt & 1) * BUF;
             const int l = i % S::N;
+            if constexpr (!LISTED) {
+                const int k = kt * KR + l * S::STEP;
+                const bool live = k < below;
+                if (i < S::N) sy.issue(buf, ly + (uint64_t)(unsigned)k * p.lddy, live, wy, l);
+                else sx.issue(buf + BT * STAGE_BYTES, lx + (uint64_t)(unsigned)k * p.ldx, live, wx, l);
+                return;
+            }
             const bool live = at[l] >= 0;
             if (i < S::N) sy.issue(buf, p.dy + (uint64_t)(unsigned)pick(p.m_dy, at[l], row_of(kt, l)) * p.lddy, live, wy, l);
             else sx.issue(buf + BT * STAGE_BYTES, p.x + (uint64_t)(unsigned)pick(p.m_x, p.by_copies(at[l]), row_of(kt, l)) * p.ldx, live, wx, l);
@@ -613,7 +637,7 @@ __global__ __launch_bounds__(WN * WK * 64, WN * WK * 64 >= 512 ? 2 : 1) void bnn
             sy.commit(buf);
             sx.commit(buf + BT * STAGE_BYTES);
         };
-        fetch(0);
+        if constexpr (LISTED) fetch(0);
         tile_loop<T, FK, FN, (FK + FN) * (sizeof(T) == 4 ? 4 : 2), 2 * S::N, DMA>(KT, acc, before, issue, commit,
             [&](int kt, int st, int i, u32x4 (&fb)[FK], u32x4 (&fa)[FN]) {
                 const char* a = smem + (kt & 1) * BUF;

@@ -131,20 +131,25 @@ inline ReducePlan reduce_plan(int64_t P, int64_t G, int64_t N, int64_t K, bool f
     const auto tiles = [&](int b) { return G * ceil_div(N, b) * ceil_div(K, b); };
     if (!f32 && tiles(256) >= 192) return {256, 1};
     if (tiles(128) >= 192) return {128, 1};
-    // about two rounds of four workgroups per CU, at least 256 rows each
-    return {64, (int)std::max<int64_t>(1, std::min<int64_t>({2048 / tiles(64), P / G / 256, 16}))};
+    // about two rounds of four workgroups per CU, at least 128 rows each
+    return {64, (int)std::max<int64_t>(1, std::min<int64_t>({2048 / tiles(64), P / G / 128, 16}))};
 }
 
-template <typename T, int BT, int WN, int WK, bool DMA>
-int launch_reduce_tile(ReduceParams p, hipStream_t st) {
+template <typename T, int BT, int WN, int WK, bool DMA, bool LISTED>
+int launch_reduce_form(ReduceParams p, hipStream_t st) {
     p.tiles_k = (int32_t)ceil_div(p.K, BT);
     const int64_t tiles = ceil_div(p.N, BT) * (p.tiles_k + (p.db ? 1 : 0));
     if (tiles > 0x7fffffffLL || p.G > 65535) return fail(BNN_ERR_RANGE, "dW takes up to 65535 members");
-    constexpr auto* kern = &bnn_grouped_dw_kernel<T, T, BT, WN, WK, DMA>;
+    constexpr auto* kern = &bnn_grouped_dw_kernel<T, T, BT, WN, WK, DMA, LISTED>;
     allow_big_lds<kern>();
     hipLaunchKernelGGL(*kern, dim3((unsigned)tiles, (unsigned)p.G, (unsigned)p.splits), dim3(WN * WK * 64), (size_t)4 * BT * STAGE_BYTES, st, p);
     HIP_TRY(hipGetLastError());
     return 0;
+}
+
+template <typename T, int BT, int WN, int WK, bool DMA>
+int launch_reduce_tile(const ReduceParams& p, hipStream_t st) {
+    return p.list ? launch_reduce_form<T, BT, WN, WK, DMA, true>(p, st) : launch_reduce_form<T, BT, WN, WK, DMA, false>(p, st);
 }
 
 template <typename T>

@@ -179,13 +179,16 @@ __global__ __launch_bounds__(256) void bnn_sum_copies_kernel(const float* __rest
     }
 }
 
-// dW / db of the splits, added in order
+// the splits' sums added in order: dW (n values), then db (nb) behind all the splits of dW
 template <typename O>
-__global__ __launch_bounds__(256) void bnn_sum_splits_kernel(const float* __restrict__ part, int splits, int64_t n, O* __restrict__ out) {
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+__global__ __launch_bounds__(256) void bnn_sum_splits_kernel(const float* __restrict__ part, int splits, int64_t n, O* __restrict__ dw, int64_t nb, O* __restrict__ db) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n + nb; i += (int64_t)gridDim.x * 256) {
+        const bool w = i < n;
+        const int64_t at = w ? i : splits * n + (i - n), step = w ? n : nb;
         float s = 0.0f;
-        for (int c = 0; c < splits; ++c) s += part[c * n + i];
-        out[i] = (O)s;
+        for (int c = 0; c < splits; ++c) s += part[at + c * step];
+        if (w) dw[i] = (O)s;
+        else db[i - n] = (O)s;
     }
 }
 
@@ -324,8 +327,8 @@ int bnn_grouped_linear_dw(const bnn_grouped* q, const void* dy, const void* x, v
     p.offsets = q->offsets;
     p.ldx = (uint32_t)(q->x_row * es); p.lddy = (uint32_t)(q->y_row * es);
     p.P = (int32_t)(q->rows * q->copies); p.G = q->members; p.N = q->outputs; p.K = q->inputs;
-    p.m_x = q->gather ? -1 : 0; p.m_dy = q->scatter ? -1 : 0; p.m_list = p.m_x | p.m_dy;
-    p.list = p.m_list ? q->order : q->offsets;
+    p.m_x = q->gather ? -1 : 0; p.m_dy = q->scatter ? -1 : 0;
+    p.list = p.m_x | p.m_dy ? q->order : nullptr;
     while ((1LL << p.shift) < q->copies) ++p.shift;   // pair / copies = (2 pair * magic >> 32) >> shift, exact below 2^31: magic = ceil(2^(31 + shift) / copies)
     p.magic = (uint32_t)(((1ULL << (31 + p.shift)) + q->copies - 1) / q->copies);
     const ReducePlan plan = plan_of(q);
@@ -338,12 +341,8 @@ int bnn_grouped_linear_dw(const bnn_grouped* q, const void* dy, const void* x, v
     const hipStream_t st = (hipStream_t)stream;
     const auto join = [&](auto tag) -> int {
         using O = typename decltype(tag)::type;
-        hipLaunchKernelGGL(bnn_sum_splits_kernel<O>, dim3(sweep_blocks(n)), dim3(256), 0, st, part, p.splits, n, (O*)dw);
+        hipLaunchKernelGGL(bnn_sum_splits_kernel<O>, dim3(sweep_blocks(n + (db ? nb : 0))), dim3(256), 0, st, part, p.splits, n, (O*)dw, db ? nb : 0, (O*)db);
         HIP_TRY(hipGetLastError());
-        if (db) {
-            hipLaunchKernelGGL(bnn_sum_splits_kernel<O>, dim3(sweep_blocks(nb)), dim3(256), 0, st, part + (int64_t)p.splits * n, p.splits, nb, (O*)db);
-            HIP_TRY(hipGetLastError());
-        }
         return 0;
     };
     if (q->dtype == BNN_TYPE_F32) return join(Tag<float>{});
