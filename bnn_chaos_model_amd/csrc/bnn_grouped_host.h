@@ -28,10 +28,11 @@ inline int64_t likely_tiles(const RowsParams& p, int BM) {
     return p.offsets ? std::max<int64_t>(used, p.P / BM + used / 2) : ceil_div(p.P, BM);
 }
 
-inline int set_grid(RowsParams& p, int BM, int BN, int band) {
+// a grid has fewer than 2^32 threads along x
+inline int set_grid(RowsParams& p, int BM, int BN, int band, int threads) {
     p.tiles_n = (int32_t)ceil_div(p.N, BN);
     const int64_t nblk = row_tiles(p, BM) * p.tiles_n;
-    if (nblk > 0x7fffffffLL) return fail(BNN_ERR_RANGE, "too many tiles for one launch");
+    if (nblk * threads > 0xffffffffLL) return fail(BNN_ERR_RANGE, "too many tiles for one launch");
     p.nblk = (int32_t)nblk;
     p.band = band;
     return 0;
@@ -39,7 +40,7 @@ inline int set_grid(RowsParams& p, int BM, int BN, int band) {
 
 template <typename T, typename O, int BM, int BN, int WM, int WN, bool WFC, bool DMA>
 int launch_rows_tile(RowsParams p, hipStream_t st) {
-    if (int rc = set_grid(p, BM, BN, 8)) return rc;
+    if (int rc = set_grid(p, BM, BN, 8, WM * WN * 64)) return rc;
     constexpr auto* kern = &bnn_grouped_kernel<T, O, BM, BN, WM, WN, WFC, DMA>;
     allow_big_lds<kern>();
     hipLaunchKernelGGL(*kern, dim3((unsigned)p.nblk), dim3(WM * WN * 64), (size_t)2 * (BM + BN) * STAGE_BYTES, st, p);
@@ -49,7 +50,7 @@ int launch_rows_tile(RowsParams p, hipStream_t st) {
 
 template <typename T, typename O, int FM, int FN, int U, bool VEC>
 int launch_rows_few(RowsParams p, hipStream_t st) {
-    if (int rc = set_grid(p, 16 * FM, 16 * FN, 1)) return rc;
+    if (int rc = set_grid(p, 16 * FM, 16 * FN, 1, 512)) return rc;
     constexpr auto* kern = &bnn_grouped_few_kernel<T, O, FM, FN, U, VEC>;
     allow_big_lds<kern>();
     hipLaunchKernelGGL(*kern, dim3((unsigned)p.nblk), dim3(512), (size_t)8 * FM * FN * 64 * 16, st, p);
@@ -72,7 +73,7 @@ int launch_rows_short(RowsParams p, hipStream_t st) {
     int64_t room = 512;
     while (room <= loss) room += 512;
     p.block_rows = (int32_t)std::max<int64_t>(64, ceil_div(ceil_div(p.P * tiles_n, room - loss / 2), 64) * 64);
-    if (int rc = set_grid(p, p.block_rows, 16 * FN, 1)) return rc;
+    if (int rc = set_grid(p, p.block_rows, 16 * FN, 1, 256)) return rc;
     hipLaunchKernelGGL((bnn_grouped_short_kernel<T, O, FN, ST>), dim3((unsigned)p.nblk), dim3(256), 0, st, p);
     HIP_TRY(hipGetLastError());
     return 0;
@@ -139,7 +140,8 @@ template <typename T, int BT, int WN, int WK, bool DMA, bool LISTED>
 int launch_reduce_form(ReduceParams p, hipStream_t st) {
     p.tiles_k = (int32_t)ceil_div(p.K, BT);
     const int64_t tiles = ceil_div(p.N, BT) * (p.tiles_k + (p.db ? 1 : 0));
-    if (tiles > 0x7fffffffLL || p.G > 65535) return fail(BNN_ERR_RANGE, "dW takes up to 65535 members");
+    if (p.G > 65535) return fail(BNN_ERR_RANGE, "dW takes up to 65535 members");
+    if (tiles * WN * WK * 64 > 0xffffffffLL) return fail(BNN_ERR_RANGE, "too many tiles for one launch");
     constexpr auto* kern = &bnn_grouped_dw_kernel<T, T, BT, WN, WK, DMA, LISTED>;
     allow_big_lds<kern>();
     hipLaunchKernelGGL(*kern, dim3((unsigned)tiles, (unsigned)p.G, (unsigned)p.splits), dim3(WN * WK * 64), (size_t)4 * BT * STAGE_BYTES, st, p);

@@ -209,11 +209,11 @@ unsigned sweep_blocks(int64_t n) { return (unsigned)std::min<int64_t>(std::max<i
 
 ReducePlan plan_of(const bnn_grouped* q) { return reduce_plan(q->rows * q->copies, q->members, q->outputs, q->inputs, q->dtype == BNN_TYPE_F32); }
 
-int check_grouped(const bnn_grouped* q, bool int8) {
+int check_grouped(const bnn_grouped* q) {
     if (!q) return fail(BNN_ERR_INVALID, "grouped descriptor is NULL");
     if (q->dtype < BNN_TYPE_F32 || q->dtype > BNN_TYPE_F16) return fail(BNN_ERR_INVALID, "dtype must be one of bnn_dtype");
     if (q->rows < 0 || q->copies < 1 || q->members < 1 || q->inputs < 1 || q->outputs < 1) return fail(BNN_ERR_INVALID, "bad rows / copies / members / inputs / outputs");
-    if (q->rows > 0x7fffffffLL / q->copies) return fail(BNN_ERR_RANGE, "rows x copies must stay below 2^31");
+    if (q->rows >= (1LL << 30) / q->copies + ((1LL << 30) % q->copies != 0)) return fail(BNN_ERR_RANGE, "rows x copies must stay below 2^30");
     if (q->inputs > (1 << 24) || q->outputs > (1 << 24) || q->members > (1 << 24)) return fail(BNN_ERR_RANGE, "members, inputs and outputs must stay below 2^24");
     if (q->x_row < 0 || q->y_row < 0 || q->x_row > (1 << 28) || q->y_row > (1 << 28)) return fail(BNN_ERR_RANGE, "rows must be less than 2^28 elements apart");
     if ((q->gather || q->scatter) && q->rows && !q->order) return fail(BNN_ERR_INVALID, "gather / scatter need order");
@@ -233,7 +233,7 @@ size_t bnn_group_rows_workspace_bytes(int64_t pairs, int32_t members) {
 int bnn_group_rows_i32(const int32_t* member, int64_t pairs, int32_t members, int32_t* order, int32_t* offsets, void* workspace, void* stream) {
     if (pairs < 0 || members < 1) return fail(BNN_ERR_INVALID, "bad pairs / members");
     if (members > GROUP_MAX_MEMBERS) return fail(BNN_ERR_UNSUPPORTED, "group_rows sorts by up to 4096 members");
-    if (pairs > 0x7fffffffLL) return fail(BNN_ERR_RANGE, "pairs must stay below 2^31");
+    if (pairs >= (1LL << 30)) return fail(BNN_ERR_RANGE, "pairs must stay below 2^30");
     if (!offsets || (pairs && (!member || !order))) return fail(BNN_ERR_INVALID, "NULL argument");
     const int64_t nb = (pairs + GROUP_CHUNK - 1) / GROUP_CHUNK;
     if (nb > 1 && !workspace) return fail(BNN_ERR_INVALID, "workspace is NULL");
@@ -268,7 +268,7 @@ int bnn_group_rows_i32(const int32_t* member, int64_t pairs, int32_t members, in
 }
 
 int bnn_grouped_linear(const bnn_grouped* q, const void* x, const void* w, const void* bias, void* y, void* stream) {
-    if (int rc = check_grouped(q, false)) return rc;
+    if (int rc = check_grouped(q)) return rc;
     if (q->rows == 0) return 0;
     if (!x || !w || !y || !q->offsets) return fail(BNN_ERR_INVALID, "NULL argument");
     const int es = type_size(q->dtype);
@@ -287,7 +287,7 @@ size_t bnn_grouped_linear_dx_workspace_bytes(const bnn_grouped* q) {
 }
 
 int bnn_grouped_linear_dx(const bnn_grouped* q, const void* dy, const void* w, void* dx, void* workspace, void* stream) {
-    if (int rc = check_grouped(q, false)) return rc;
+    if (int rc = check_grouped(q)) return rc;
     if (q->rows == 0) return 0;
     if (!dy || !w || !dx || !q->offsets) return fail(BNN_ERR_INVALID, "NULL argument");
     const int es = type_size(q->dtype);
@@ -319,7 +319,7 @@ size_t bnn_grouped_linear_dw_workspace_bytes(const bnn_grouped* q) {
 }
 
 int bnn_grouped_linear_dw(const bnn_grouped* q, const void* dy, const void* x, void* dw, void* db, void* workspace, void* stream) {
-    if (int rc = check_grouped(q, false)) return rc;
+    if (int rc = check_grouped(q)) return rc;
     if (!dw || !q->offsets || (q->rows && (!dy || !x))) return fail(BNN_ERR_INVALID, "NULL argument");
     const int es = type_size(q->dtype);
     ReduceParams p{};

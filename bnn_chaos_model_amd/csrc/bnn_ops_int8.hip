@@ -278,7 +278,7 @@ int check_int8(const bnn_grouped* q) {
     if (!q) return fail(BNN_ERR_INVALID, "grouped descriptor is NULL");
     if (q->dtype < BNN_TYPE_F32 || q->dtype > BNN_TYPE_F16) return fail(BNN_ERR_INVALID, "dtype must be one of bnn_dtype");
     if (q->rows < 0 || q->copies < 1 || q->members < 1 || q->inputs < 1 || q->outputs < 1) return fail(BNN_ERR_INVALID, "bad rows / copies / members / inputs / outputs");
-    if (q->rows > 0x7fffffffLL / q->copies) return fail(BNN_ERR_RANGE, "rows x copies must stay below 2^31");
+    if (q->rows >= (1LL << 30) / q->copies + ((1LL << 30) % q->copies != 0)) return fail(BNN_ERR_RANGE, "rows x copies must stay below 2^30");
     if (q->outputs > (1 << 24) || q->members > (1 << 24)) return fail(BNN_ERR_RANGE, "members and outputs must stay below 2^24");
     if (q->inputs > 131072) return fail(BNN_ERR_RANGE, "the 32-bit sums hold up to 131072 products of 8-bit integers");   // 2^17 * 127^2 < 2^31
     if (q->rows == 0) return 0;
@@ -315,12 +315,17 @@ int bnn_quantize_rows(const void* x, int32_t dtype, int64_t rows, int32_t K, int
         // that a wave would not hold
         const int64_t kbytes = (int64_t)K * sizeof(T);
         const int tpr = rows < 2048 || kbytes > 64 * 8 * CHUNK ? 256 : kbytes <= 1024 ? 16 : 64;
-        const unsigned nblk = (unsigned)((rows + 256 / tpr - 1) / (256 / tpr));
-        if (kbytes < CHUNK) hipLaunchKernelGGL(bnn_quantize_short_rows_kernel<T>, dim3((unsigned)((rows + 255) / 256)), dim3(256), 0, st, xb, ldx, rows, K, q, q_row, scale);
-        else if (tpr == 16) hipLaunchKernelGGL((bnn_quantize_rows_kernel<T, 16>), dim3(nblk), dim3(256), 0, st, xb, ldx, rows, K, q, q_row, scale);
-        else if (tpr == 64) hipLaunchKernelGGL((bnn_quantize_rows_kernel<T, 64>), dim3(nblk), dim3(256), 0, st, xb, ldx, rows, K, q, q_row, scale);
-        else hipLaunchKernelGGL((bnn_quantize_rows_kernel<T, 256>), dim3(nblk), dim3(256), 0, st, xb, ldx, rows, K, q, q_row, scale);
-        HIP_TRY(hipGetLastError());
+        for (int64_t r0 = 0; r0 < rows; r0 += 1 << 22) {   // (a grid has fewer than 2^32 threads)
+            const int64_t n = std::min<int64_t>(rows - r0, 1 << 22);
+            const unsigned nblk = (unsigned)((n + 256 / tpr - 1) / (256 / tpr));
+            const char* xr = xb + r0 * ldx;
+            int8_t* qr = q + r0 * q_row;
+            if (kbytes < CHUNK) hipLaunchKernelGGL(bnn_quantize_short_rows_kernel<T>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, xr, ldx, n, K, qr, q_row, scale + r0);
+            else if (tpr == 16) hipLaunchKernelGGL((bnn_quantize_rows_kernel<T, 16>), dim3(nblk), dim3(256), 0, st, xr, ldx, n, K, qr, q_row, scale + r0);
+            else if (tpr == 64) hipLaunchKernelGGL((bnn_quantize_rows_kernel<T, 64>), dim3(nblk), dim3(256), 0, st, xr, ldx, n, K, qr, q_row, scale + r0);
+            else hipLaunchKernelGGL((bnn_quantize_rows_kernel<T, 256>), dim3(nblk), dim3(256), 0, st, xr, ldx, n, K, qr, q_row, scale + r0);
+            HIP_TRY(hipGetLastError());
+        }
         return 0;
     };
     if (dtype == BNN_TYPE_F32) return launch(Tag<float>{});
@@ -362,7 +367,7 @@ int bnn_int8_linear_rows(const bnn_grouped* q, const void* x, int32_t x_dtype, v
             using XT = typename decltype(xt)::type;
             using O = typename decltype(ot)::type;
             p.vec = p.N % 4 == 0 && aligned(p.ldy, 4 * sizeof(O)) && aligned(p.y, 4 * sizeof(O));
-            if (int rc = set_grid(p, 16, 16, 1)) return rc;
+            if (int rc = set_grid(p, 16, 16, 1, 512)) return rc;
             constexpr auto* kern = &bnn_int8_handful_kernel<XT, O>;
             allow_big_lds<kern>();
             hipLaunchKernelGGL(*kern, dim3((unsigned)p.nblk), dim3(512), lds, (hipStream_t)stream, p, (int)((ld + 63) / 64 * 64 + 16));

@@ -16,11 +16,18 @@ from . import _native as N
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _INT8_MAX_INPUTS = 131072   # of 32-bit sums of products of 8-bit integers
 
+_FLOATS = tuple(_TYPES)
+
 # order int32 [pairs]: pair (row * copies + copy) at every grouped row; offsets int32 [members + 1]: first grouped row of every member;
 # shape: that of the member indices, (rows,) or (rows, copies)
 RowGroups = namedtuple("RowGroups", "order offsets shape")
 # values int8 [..., K], scale float32 [...]: the numbers values * scale[..., None]
 QuantRows = namedtuple("QuantRows", "values scale")
+
+
+class _Sorted(RowGroups):
+    """What group_rows returns: its index tensors need no second look at every call."""
+    __slots__ = ()
 
 
 def _gpu(t, name, dtypes):
@@ -38,10 +45,12 @@ def _same_device(dev, name, t):
 def _run(dev, fn, *args):
     """A native call with device `dev` current (one process may drive several), on torch's current stream of it."""
     if dev == N.current_device():
-        N.check(fn(*args, N.stream_ptr(dev)))
+        rc = fn(*args, N.stream_ptr(dev))
     else:
         with torch.cuda.device(dev):
-            N.check(fn(*args, N.stream_ptr(dev)))
+            rc = fn(*args, N.stream_ptr(dev))
+    if rc < 0:
+        N.check(rc)
 
 
 def _addr(t):
@@ -69,23 +78,24 @@ def group_rows(member, n_members):
     member: int32 [rows] or [rows, copies], the member(s) that evaluate each row; values outside [0, n_members) mean nobody (padding): those
     pairs come last, and the layers below give them zeros.  n_members <= 4096.  One launch up to 4096 pairs, three beyond."""
     _gpu(member, "member", (torch.int32,))
-    if member.dim() not in (1, 2):
+    shape = tuple(member.shape)
+    if len(shape) not in (1, 2):
         raise ValueError("member must be [rows] or [rows, copies]")
     n_members = int(n_members)
     if not 1 <= n_members <= 4096:
         raise ValueError("n_members must lie in 1 .. 4096")
-    if member.dim() == 2 and member.shape[1] < 1:
+    if len(shape) == 2 and shape[1] < 1:
         raise ValueError("member must hold at least one copy per row")
     P = member.numel()
-    if P >= 2 ** 31:
-        raise ValueError("rows x copies must stay below 2^31")
+    if P >= 1 << 30:
+        raise ValueError("rows x copies must stay below 2^30")
     m = member.contiguous()
     order = m.new_empty(P)
     offsets = m.new_empty(n_members + 1)
     nbytes = 0 if P <= 4096 else N.lib().bnn_group_rows_workspace_bytes(P, n_members)
     ws = m.new_empty(nbytes // 4) if nbytes else None
     _run(m.get_device(), N.lib().bnn_group_rows_i32, m.data_ptr(), P, n_members, order.data_ptr(), offsets.data_ptr(), _addr(ws))
-    return RowGroups(order, offsets, tuple(member.shape))
+    return _Sorted(order, offsets, shape)
 
 
 def _check_groups(groups, x, G, gather, what="x"):
@@ -93,14 +103,16 @@ def _check_groups(groups, x, G, gather, what="x"):
     if not isinstance(groups, RowGroups):
         raise TypeError("groups must be the RowGroups that group_rows returns")
     order, offsets, shape = groups
-    _gpu(order, "groups.order", (torch.int32,))
-    _gpu(offsets, "groups.offsets", (torch.int32,))
     dev = x.get_device()
-    _same_device(dev, "groups.order", order)
-    _same_device(dev, "groups.offsets", offsets)
     rows, copies = shape if len(shape) == 2 else (shape[0], 1)
-    if order.numel() != rows * copies or not order.is_contiguous() or not offsets.is_contiguous():
-        raise ValueError("groups.order must be contiguous and hold one entry per (row, copy) pair")
+    if type(groups) is not _Sorted:
+        _gpu(order, "groups.order", (torch.int32,))
+        _gpu(offsets, "groups.offsets", (torch.int32,))
+        _same_device(dev, "groups.offsets", offsets)
+        if order.numel() != rows * copies or not order.is_contiguous() or not offsets.is_contiguous():
+            raise ValueError("groups.order must be contiguous and hold one entry per (row, copy) pair")
+    if order.get_device() != dev:
+        _same_device(dev, "groups.order", order)
     if offsets.numel() != G + 1:
         raise ValueError(f"groups are over {offsets.numel() - 1} members, the weights over {G}")
     want = rows if gather else rows * copies
@@ -114,31 +126,34 @@ def _out_shape(groups, n_out, scatter):
 
 
 def _check_linear(x, weight, groups, bias, gather):
-    _gpu(x, "x", tuple(_TYPES))
-    _gpu(weight, "weight", (x.dtype,))
-    if x.dim() != 2 or weight.dim() != 3 or weight.shape[2] != x.shape[1] or min(weight.shape) < 1:
+    _gpu(x, "x", _FLOATS)
+    dtype, dev = x.dtype, x.get_device()
+    _gpu(weight, "weight", (dtype,))
+    G, n_out, n_in = weight.shape if weight.dim() == 3 else (0, 0, 0)
+    if x.dim() != 2 or n_in != x.shape[1] or G < 1 or n_out < 1 or n_in < 1:
         raise ValueError("x must be [rows, K] and weight [members, N, K]")
-    if max(weight.shape) > 1 << 24:
+    if max(G, n_out, n_in) > 1 << 24:
         raise ValueError("members, inputs and outputs must stay below 2^24")
-    G, n_out, _ = weight.shape
+    _same_device(dev, "weight", weight)
     if bias is not None:
-        _gpu(bias, "bias", (x.dtype,))
-        if tuple(bias.shape) != (G, n_out):
+        _gpu(bias, "bias", (dtype,))
+        if bias.shape != (G, n_out):
             raise ValueError(f"bias must be [{G}, {n_out}]")
-        _same_device(x.get_device(), "bias", bias)
-    _same_device(x.get_device(), "weight", weight)
+        _same_device(dev, "bias", bias)
     return _check_groups(groups, x, G, gather)
 
 
 def _descriptor(groups, rows, copies, dtype, weight, x_row, y_row, gather, scatter, relu=False):
     G, n_out, n_in = weight.shape
-    return N.BnnGrouped(rows, copies, G, n_in, n_out, _TYPES[dtype], int(bool(gather)), int(bool(scatter)), int(bool(relu)), x_row, y_row,
-                        weight.stride(0) if G > 1 else 0, weight.stride(1) if n_out > 1 else n_in, _addr(groups.order), _addr(groups.offsets))
+    member, row, _ = weight.stride()
+    return N.BnnGrouped(rows, copies, G, n_in, n_out, _TYPES[dtype], 1 if gather else 0, 1 if scatter else 0, 1 if relu else 0, x_row, y_row,
+                        member if G > 1 else 0, row if n_out > 1 else n_in, groups.order.data_ptr(), groups.offsets.data_ptr())
 
 
 def _linear(x, weight, groups, bias, relu, gather, scatter, rows, copies):
     x, weight = _rows2d(x), _layers(weight)
-    bias = None if bias is None else bias.contiguous()
+    if bias is not None and not bias.is_contiguous():
+        bias = bias.contiguous()
     y = x.new_empty(_out_shape(groups, weight.shape[1], scatter))
     q = _descriptor(groups, rows, copies, x.dtype, weight, _row_stride(x), weight.shape[1], gather, scatter, relu)
     _run(x.get_device(), N.lib().bnn_grouped_linear, q, x.data_ptr(), weight.data_ptr(), _addr(bias), y.data_ptr())
@@ -210,21 +225,26 @@ def grouped_linear(x, weight, groups, bias=None, relu=False, gather=False, scatt
     gather=True: x holds the batch's rows, each read by the member(s) its indices name; False: x [pairs, K] is already in grouped order.
     scatter=True: y comes in the batch's order, [rows, N] or [rows, copies, N]; False: in grouped order, [pairs, N] -- so a chain of layers
     gathers in the first, scatters in the last and permutes nothing in between.  Rows of nobody: zero.
+    Under stream capture call it in torch.no_grad() (a captured training step: grouped_linear_grads for its backward pass).
     x and weight may be strided as long as the elements along K are neighbours (a layer's slice of flat parameter vectors [members, d]).
     Sums are fp32 (float32 operands: exact fp32 products), rounded once to the operands' type."""
     rows, copies = _check_linear(x, weight, groups, bias, gather)
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("grouped_linear records no autograd graph under stream capture: autograd would join the capture with the streams of "
+                               "earlier graphs of the same leaves.  Capture it under torch.no_grad() with grouped_linear_grads as the backward pass")
         return _GroupedLinear.apply(x, weight, bias, groups, relu, gather, scatter, rows, copies)
     return _linear(x, weight, groups, bias, relu, gather, scatter, rows, copies)
 
 
 def _check_quantize(x):
-    _gpu(x, "x", tuple(_TYPES))
-    if x.dim() < 1 or x.shape[-1] < 1:
+    _gpu(x, "x", _FLOATS)
+    K = x.shape[-1] if x.dim() else 0
+    if K < 1:
         raise ValueError("x must be [..., K] with K >= 1")
-    if x.shape[-1] > 1 << 24 or x.numel() // x.shape[-1] >= 2 ** 31:
+    if K > 1 << 24 or x.numel() >= K << 31:
         raise ValueError("rows must stay below 2^31, their length below 2^24")
-    if torch.is_grad_enabled() and x.requires_grad:
+    if x.requires_grad and torch.is_grad_enabled():
         raise NotImplementedError("8-bit rows have no gradient: detach x")
 
 
@@ -233,10 +253,11 @@ def quantize_rows(x):
     channel of a weight [N, K] / [members, N, K]), values = x / scale rounded half to even, exactly.  A row of zeros has scale 0; a row that holds
     NaN or an infinity has scale NaN, so that whatever is computed from it is NaN."""
     _check_quantize(x)
-    K = x.shape[-1]
-    x2 = _rows2d(x if x.dim() == 2 else x.reshape(-1, K))
-    values = x.new_empty(x.shape, dtype=torch.int8)
-    scale = x.new_empty(x.shape[:-1], dtype=torch.float32)
+    shape = x.shape
+    K = shape[-1]
+    x2 = _rows2d(x if len(shape) == 2 else x.reshape(-1, K))
+    values = torch.empty(shape, dtype=torch.int8, device=x.device)
+    scale = torch.empty(shape[:-1], dtype=torch.float32, device=x.device)
     _run(x.get_device(), N.lib().bnn_quantize_rows, x2.data_ptr(), _TYPES[x.dtype], x2.shape[0], K, _row_stride(x2), values.data_ptr(), K, scale.data_ptr())
     return QuantRows(values, scale)
 
@@ -249,8 +270,7 @@ def int8_linear(x, weight, groups=None, bias=None, relu=False, gather=False, sca
     type; float32 for QuantRows).  Inference only; K <= 131072."""
     quant = isinstance(x, QuantRows)
     if quant:
-        xq, xs = _gpu(x.values, "x.values", (torch.int8,)), _gpu(x.scale, "x.scale", (torch.float32,))
-        rows_of = xq
+        rows_of, xs = _gpu(x.values, "x.values", (torch.int8,)), _gpu(x.scale, "x.scale", (torch.float32,))
     else:
         _check_quantize(x)
         rows_of = x
@@ -260,46 +280,57 @@ def int8_linear(x, weight, groups=None, bias=None, relu=False, gather=False, sca
     if not isinstance(weight, QuantRows):
         raise TypeError("weight must be the QuantRows that quantize_rows returns")
     wq, ws = _gpu(weight.values, "weight.values", (torch.int8,)), _gpu(weight.scale, "weight.scale", (torch.float32,))
-    want = 2 if groups is None else 3
-    if rows_of.dim() != 2 or wq.dim() != want or wq.shape[-1] != rows_of.shape[1] or min(wq.shape) < 1:
+    shape = wq.shape
+    if len(shape) != (2 if groups is None else 3) or rows_of.dim() != 2 or shape[-1] != rows_of.shape[1] or min(shape) < 1:
         raise ValueError("x must be [rows, K], weight [N, K] without groups or [members, N, K] with them")
-    if wq.shape[-1] > _INT8_MAX_INPUTS:
+    if wq.stride(-1) != 1 and shape[-1] > 1:
+        wq = wq.contiguous()
+    if groups is None:
+        (n_out, n_in), G, strides = shape, 1, (0, wq.stride(0))
+    else:
+        (G, n_out, n_in), strides = shape, wq.stride()
+    if n_in > _INT8_MAX_INPUTS:
         raise ValueError(f"K must not exceed {_INT8_MAX_INPUTS}: the sums are 32-bit integers")
-    if max(wq.shape) > 1 << 24:
+    if G > 1 << 24 or n_out > 1 << 24:
         raise ValueError("members and outputs must stay below 2^24")
-    if tuple(ws.shape) != tuple(wq.shape[:-1]) or (quant and tuple(xs.shape) != (xq.shape[0],)):
+    if ws.shape != shape[:-1] or (quant and xs.shape != rows_of.shape[:1]):
         raise ValueError("scales must have their values' shape without the last dimension")
+    dev = rows_of.get_device()
+    _same_device(dev, "weight.values", wq)
+    _same_device(dev, "weight.scale", ws)
     if bias is not None:
         _gpu(bias, "bias", (dtype,))
-        if tuple(bias.shape) != tuple(wq.shape[:-1]):
-            raise ValueError(f"bias must be {list(wq.shape[:-1])}")
-        if torch.is_grad_enabled() and bias.requires_grad:
+        if bias.shape != shape[:-1]:
+            raise ValueError(f"bias must be {list(shape[:-1])}")
+        if bias.requires_grad and torch.is_grad_enabled():
             raise NotImplementedError("the 8-bit layer has no gradient: detach bias")
+        _same_device(dev, "bias", bias)
         bias = bias.contiguous()
-    dev = rows_of.get_device()
-    for name, t in (("weight.values", wq), ("weight.scale", ws)) + ((("bias", bias),) if bias is not None else ()) + ((("x.scale", xs),) if quant else ()):
-        _same_device(dev, name, t)
     if groups is None:
         if gather or scatter:
             raise ValueError("gather / scatter need groups")
-        wq, rows, copies = wq[None], rows_of.shape[0], 1
-        if rows >= 2 ** 31:
-            raise ValueError("rows must stay below 2^31")
-        shape = (rows, wq.shape[1])
+        rows, copies, order, offsets = rows_of.shape[0], 1, None, None
+        if rows >= 1 << 30:
+            raise ValueError("rows must stay below 2^30")
+        out = (rows, n_out)
     else:
-        rows, copies = _check_groups(groups, rows_of, wq.shape[0], gather)
-        shape = _out_shape(groups, wq.shape[1], scatter)
-    rows_of = _rows2d(rows_of)
-    wq, ws = _layers(wq), ws.contiguous()
-    y = rows_of.new_empty(shape, dtype=dtype)
-    G, n_out, n_in = wq.shape
-    q = N.BnnGrouped(rows, copies, G, n_in, n_out, _TYPES[dtype], int(bool(gather)), int(bool(scatter)), int(bool(relu)), _row_stride(rows_of), n_out,
-                     wq.stride(0) if G > 1 else 0, wq.stride(1) if n_out > 1 else n_in, None if groups is None else _addr(groups.order),
-                     None if groups is None else _addr(groups.offsets))
+        rows, copies = _check_groups(groups, rows_of, G, gather)
+        order, offsets = groups.order.data_ptr(), groups.offsets.data_ptr()
+        out = _out_shape(groups, n_out, scatter)
+    rows_of, ws = _rows2d(rows_of), ws.contiguous()
+    y = rows_of.new_empty(out, dtype=dtype)
+    q = N.BnnGrouped(rows, copies, G, n_in, n_out, _TYPES[dtype], 1 if gather else 0, 1 if scatter else 0, 1 if relu else 0, _row_stride(rows_of), n_out,
+                     strides[0] if G > 1 else 0, strides[1] if n_out > 1 else n_in, order, offsets)
     if quant:
+        _same_device(dev, "x.scale", xs)
         xs = xs.contiguous()
         _run(dev, N.lib().bnn_int8_linear, q, rows_of.data_ptr(), xs.data_ptr(), wq.data_ptr(), ws.data_ptr(), _addr(bias), y.data_ptr())
     else:
-        space = rows_of.new_empty(max(N.lib().bnn_int8_linear_rows_workspace_bytes(q), 1), dtype=torch.uint8)   # of the codes
+        space = rows_of.new_empty(max(int8_rows_workspace(rows_of.shape[0], n_in), 1), dtype=torch.uint8)
         _run(dev, N.lib().bnn_int8_linear_rows, q, rows_of.data_ptr(), _TYPES[rows_of.dtype], space.data_ptr(), wq.data_ptr(), ws.data_ptr(), _addr(bias), y.data_ptr())
     return y
+
+
+def int8_rows_workspace(rows, n_in):
+    """Bytes that the codes and scales of `rows` rows take (bnn_int8_linear_rows_workspace_bytes, without the call)."""
+    return rows * (-(-n_in // 16) * 16 + 4)

@@ -359,7 +359,8 @@ int bnn_multiswag_bands_f32(const bnn_plan* plan, const bnn_grid* grid, const fl
  *
  * A PAIR is (row, copy): row i of the batch is evaluated by `copies` members, pair p = i * copies + c.  bnn_group_rows_i32 sorts the pairs by
  * member, stably: order[r] = pair at grouped row r, offsets[m] = first grouped row of member m (offsets[members] = end of the last one's).
- * Pairs whose member lies outside [0, members) belong to nobody and come last; their outputs and gradients are zero.  members <= 4096 there;
+ * Pairs whose member lies outside [0, members) belong to nobody and come last; their outputs and gradients are zero.  Pairs stay below 2^30; members
+ * <= 4096 there;
  * workspace: bnn_group_rows_workspace_bytes (0: NULL is fine).
  *
  * bnn_grouped: rows of x / dx are x_row elements apart, rows of y / dy y_row elements; w(m, n, k) at m * w_member + n * w_row + k.

@@ -459,6 +459,27 @@ def test_captured_and_replayed_next_to_eager_work(ops):
             assert all(torch.equal(a, c) for a, c in zip(out, want))
 
 
+def test_autograd_under_capture_is_refused(ops):
+    """... also while an eager graph of the same leaves lives; the process and the leaves stay usable, and the plain functions capture."""
+    m, x, w, b = make(64, 3, 0, 16, 24, torch.float32, True)
+    for t in (x, w, b):
+        t.requires_grad_(True)
+    gr = ops.group_rows(m, 3)
+    alive = ops.grouped_linear(x, w, gr, bias=b, gather=True, scatter=True)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        with pytest.raises(RuntimeError, match="capture"):
+            ops.grouped_linear(x, w, gr, bias=b, gather=True, scatter=True)
+        with torch.no_grad():
+            y = ops.grouped_linear(x, w, gr, bias=b, gather=True, scatter=True)
+            grads = ops.grouped_linear_grads(torch.ones_like(y), x, w, gr, gather=True, scatter=True)
+    want = torch.autograd.grad(alive, (x, w, b), torch.ones_like(alive))
+    for _ in range(3):
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, alive) and all(torch.equal(a, c) for a, c in zip(grads, want))
+
+
 def test_on_another_stream(ops):
     m, x, w, b = make(3000, 5, 0, 128, 64, torch.float32, True)
     gr = ops.group_rows(m, 5)
