@@ -154,6 +154,46 @@ def test_grouped_linear_grads(ops, n, G, copies, K, N, dtype):
         assert only[0] is None and only[2] is None and torch.equal(only[1], dw)
 
 
+# Sizes at which each kernel form is the one chosen: tiles of 256 (with members whose last tile is a half one), 128 and 64, rows that can and cannot be
+# loaded straight into LDS, few rows a member, short rows, and for dW tiles of 256, 128 and 64 with and without row splits.
+FORMS = [(4000, 3, 264, 4096), (4001, 3, 263, 4095), (5000, 2, 264, 1024), (5001, 2, 263, 1022), (3000, 30, 64, 128), (700, 3, 2048, 2048), (701, 3, 2047, 2050),
+         (900, 3, 1024, 1024), (901, 3, 1023, 1021), (90, 2, 512, 512), (40, 1, 4096, 80), (5, 4, 2000, 200), (6, 4, 2001, 201), (4000, 9, 17, 130), (4000, 9, 41, 40),
+         (3000, 2, 9, 70), (3000, 2, 61, 200), (3001, 1, 4096, 264), (9000, 1, 72, 136)]
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("n,G,K,N", FORMS)
+def test_every_form_of_the_layer(ops, n, G, K, N, dtype):
+    """Forward, gradients (rows in the members' order and through the order) and the 8-bit layer at the sizes above."""
+    for moved in (True, False):
+        m, x, w, b = make(n, G, 0, K, N, DT[dtype], moved, seed=n + N)
+        gr = ops.group_rows(m, G)
+        xi, yi, mem = pair_view(gr, m, moved, moved)
+        y = ops.grouped_linear(x, w, gr, bias=b, gather=moved, scatter=moved)
+        want, mag = plain(x, w, b, xi, yi, mem, n)
+        within(y, want, (K + 2) * 2.0 ** -23 * mag)
+        dy = torch.randn(n, N, generator=_gen(n), device="cuda").to(x.dtype)
+        dx, dw, db = ops.grouped_linear_grads(dy, x, w, gr, gather=moved, scatter=moved)
+        wx, mx = torch.zeros(n, K, dtype=torch.float64, device="cuda"), torch.zeros(n, K, dtype=torch.float64, device="cuda")
+        for g in range(G):
+            sel = np.nonzero(mem == g)[0]
+            a, t = torch.as_tensor(xi[sel], device="cuda"), torch.as_tensor(yi[sel], device="cuda")
+            d, wg, xg = dy[t].double(), w[g].double(), x[a].double()
+            wx[a], mx[a] = d @ wg, d.abs() @ wg.abs()
+            within(dw[g], d.t() @ xg, (sel.size + 2) * 2.0 ** -23 * (d.abs().t() @ xg.abs()))
+            within(db[g], d.sum(0), (sel.size + 2) * 2.0 ** -23 * d.abs().sum(0))
+        within(dx, wx, (N + 2) * 2.0 ** -23 * mx)
+        wq = ops.quantize_rows(w)
+        q, s = ops.quantize_rows(x)
+        y8 = ops.int8_linear(x, wq, groups=gr, bias=b, relu=True, gather=moved, scatter=moved)
+        want, mag = torch.zeros(n, N, dtype=torch.float64, device="cuda"), torch.zeros(n, N, dtype=torch.float64, device="cuda")
+        for g in range(G):
+            sel = np.nonzero(mem == g)[0]
+            a, t = torch.as_tensor(xi[sel], device="cuda"), torch.as_tensor(yi[sel], device="cuda")
+            want[t], mag[t] = int8_plain(q[a], s[a], wq.values[g], wq.scale[g], b[g])
+        within(y8, want.clamp_min(0), INT8_SLACK * mag)
+
+
 def test_gradients_are_the_differences(ops):
     """Whole numbers: every sum is exact in fp32 and the layer is linear, so (L(t + h) - L(t - h)) / 2 equals the gradient's product with h exactly."""
     g = _gen(3)
