@@ -35,7 +35,7 @@ struct ReduceParams {          // dW[g] = sum over rows r of member g of dy_r x_
     int32_t P, G, N, K;
     int32_t m_x, m_dy;             // -1: row r of the grouped order is row order[r] / copies of x, row order[r] of dy; 0: row r
     uint32_t magic, shift;         // of the division by copies
-    int32_t tiles_k, splits;
+    int32_t tiles_n, tiles_k, splits;
     int32_t vec;                   // K % 4 == 0 and dw aligned to four elements
     __device__ __forceinline__ unsigned by_copies(int pair) const { return __umulhi(2u * (unsigned)pair, magic) >> shift; }
 };
@@ -522,46 +522,69 @@ __global__ __launch_bounds__(256) void bnn_grouped_short_kernel(RowsParams p) {
 }
 
 // ---- dW, db --------------------------------------------------------------------------------------------------------------------------------
-// BT outputs x BT inputs of one member per workgroup (blockIdx.y), over split blockIdx.z of the member's rows.  The workgroups in front of the first
-// input tile sum dy's columns (the bias gradient) instead.
+// BT outputs x BT inputs of one member per workgroup, over split blockIdx.y of the member's rows; further workgroups sum dy's columns, the bias
+// gradient.
 // LISTED: rows of x or dy are found through the order (else both are in grouped order, and a load's row is the wave's plus a constant).
 template <typename T, typename O, int BT, int WN, int WK, bool DMA, bool LISTED>
 __global__ __launch_bounds__(WN * WK * 64, WN * WK * 64 >= 512 ? 2 : 1) void bnn_grouped_dw_kernel(ReduceParams p) {
     constexpr int NT = WN * WK * 64, FN = BT / WN / 16, FK = BT / WK / 16, BUF = 2 * BT * STAGE_BYTES, KR = stage_k<T>();
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wn = wave / WK, wk = wave % WK;
-    const int cols = p.tiles_k + (p.db ? 1 : 0);
-    const int g = blockIdx.y, n0 = ((int)blockIdx.x / cols) * BT, tk = (int)blockIdx.x % cols - (p.db ? 1 : 0), k0 = tk * BT;
+    // the workgroups that sum dy's columns come first; behind them XCD x takes the x-th eighth of the tiles, member by member, four output tiles
+    // side by side (what runs together on an XCD shares its operands)
+    constexpr int BC = STAGE_BYTES / (int)sizeof(T);   // dy's columns per workgroup: 128 bytes of a row, for many rows in flight
+    const int ncol = (p.N + BC - 1) / BC, nbias = p.db ? p.G * ncol : 0;
+    const bool bias = (int)blockIdx.x < nbias;
+    int g, tn, tk = 0;
+    if (bias) {
+        g = (int)blockIdx.x / ncol;
+        tn = (int)blockIdx.x - g * ncol;
+    } else {
+        const int all = (int)gridDim.x - nbias, b = (int)blockIdx.x - nbias, per = all / 8, rem = all % 8, x = b % 8;
+        const int i = x * per + min(x, rem) + b / 8, each = p.tiles_n * p.tiles_k;
+        g = i / each;
+        const int in = i - g * each, band = in / (4 * p.tiles_k), at = in - band * 4 * p.tiles_k, rows = min(4, p.tiles_n - band * 4);
+        tk = at / rows;
+        tn = band * 4 + at - tk * rows;
+    }
+    const int n0 = tn * (bias ? BC : BT), k0 = tk * BT;
     int r0 = min(max(p.offsets[g], 0), p.P), r1 = min(max(p.offsets[g + 1], r0), p.P);
     if (p.splits > 1) {   // whole stages per split
         const int64_t len = (((int64_t)(r1 - r0) + p.splits - 1) / p.splits + KR - 1) / KR * KR;
-        const int64_t lo = r0 + len * blockIdx.z;
+        const int64_t lo = r0 + len * blockIdx.y;
         r0 = (int)(lo < r1 ? lo : r1);
         r1 = (int)(lo + len < r1 ? lo + len : r1);
         r1 = max(r1, r0);
     }
     const bool whole = p.splits == 1;
     const int64_t nk = (int64_t)p.N * p.K, gnk = p.G * nk;
-    if (tk < 0) {   // a thread takes one chunk of every RL-th row, four rows at a time; the RL sums meet in LDS, in order
-        constexpr int E = CHUNK / (int)sizeof(T), CW = BT / E, RL = NT / CW;
-        float* part = reinterpret_cast<float*>(smem);   // [RL][BT]
+    if (bias) {   // a thread takes one chunk of every RL-th row, U rows at a time; the RL sums meet in LDS, in order
+        constexpr int E = CHUNK / (int)sizeof(T), CW = BC / E, RL = NT / CW, U = 16;
+        float* part = reinterpret_cast<float*>(smem);   // [RL][BC]
         const int c = tid % CW, rl = tid / CW;
         const int64_t width = (int64_t)p.N * sizeof(T), byte = ((int64_t)n0 + c * E) * sizeof(T);
+        const bool inside = (int64_t)(n0 + BC) * (int64_t)sizeof(T) <= width, tail = width >= CHUNK;
         float s[E];
 #pragma unroll
         for (int e = 0; e < E; ++e) s[e] = 0.0f;
-        for (int r = r0 + rl; r < r1; r += 4 * RL) {
-            u32x4 v[4];
+        for (int r = r0 + rl; r < r1; r += U * RL) {
+            int src[U];
+            u32x4 v[U];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
+            for (int u = 0; u < U; ++u) {
                 const int row = r + u * RL;
-                int src = min(row, r1 - 1);
-                if (p.m_dy) src = p.list[src];
-                v[u] = u32x4{0, 0, 0, 0};
-                if (row < r1 && src >= 0 && src < p.P) v[u] = load_chunk<T>(p.dy + (int64_t)src * p.lddy, byte, width, (int64_t)(n0 + BT) * (int64_t)sizeof(T) <= width);
+                src[u] = LISTED && p.m_dy ? p.list[min(row, r1 - 1)] : row;
+                if (row >= r1 || src[u] >= p.P) src[u] = -1;
             }
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
+            for (int u = 0; u < U; ++u) {
+                const bool live = src[u] >= 0;
+                const char* row = live ? p.dy + (uint64_t)(unsigned)src[u] * p.lddy : (const char*)zero_chunk;
+                if (tail) v[u] = load_chunk<T>(row, live ? byte : 0, live ? width : CHUNK, inside);
+                else v[u] = load_short<T>(row, byte, live ? width : 0);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
                 T t[E];
                 __builtin_memcpy(t, &v[u], CHUNK);
 #pragma unroll
@@ -569,15 +592,15 @@ __global__ __launch_bounds__(WN * WK * 64, WN * WK * 64 >= 512 ? 2 : 1) void bnn
             }
         }
 #pragma unroll
-        for (int e = 0; e < E; ++e) part[rl * BT + c * E + e] = s[e];
+        for (int e = 0; e < E; ++e) part[rl * BC + c * E + e] = s[e];
         __syncthreads();
-        for (int i = tid; i < BT; i += NT) {
+        for (int i = tid; i < BC; i += NT) {
             const int n = n0 + i;
             float sum = part[i];
-            for (int l = 1; l < RL; ++l) sum += part[l * BT + i];
+            for (int l = 1; l < RL; ++l) sum += part[l * BC + i];
             if (n < p.N) {
                 if (whole) reinterpret_cast<O*>(p.db)[(int64_t)g * p.N + n] = (O)sum;
-                else p.part[p.splits * gnk + ((int64_t)blockIdx.z * p.G + g) * p.N + n] = sum;
+                else p.part[p.splits * gnk + ((int64_t)blockIdx.y * p.G + g) * p.N + n] = sum;
             }
         }
         return;
@@ -646,7 +669,7 @@ __global__ __launch_bounds__(WN * WK * 64, WN * WK * 64 >= 512 ? 2 : 1) void bnn
                 else fb[i - FN] = frag_fc<T, BT>(b, wk * (BT / WK) + (i - FN) * 16, st, lane);
             });
     }
-    char* dst = whole ? p.dw + g * nk * (int64_t)sizeof(O) : reinterpret_cast<char*>(p.part + blockIdx.z * gnk + g * nk);
+    char* dst = whole ? p.dw + g * nk * (int64_t)sizeof(O) : reinterpret_cast<char*>(p.part + blockIdx.y * gnk + g * nk);
 #pragma unroll
     for (int f = 0; f < FN; ++f) {
         const int n = n0 + wn * (BT / WN) + f * 16 + (lane & 15);

@@ -139,12 +139,12 @@ inline ReducePlan reduce_plan(int64_t P, int64_t G, int64_t N, int64_t K, bool f
 template <typename T, int BT, int WN, int WK, bool DMA, bool LISTED>
 int launch_reduce_form(ReduceParams p, hipStream_t st) {
     p.tiles_k = (int32_t)ceil_div(p.K, BT);
-    const int64_t tiles = ceil_div(p.N, BT) * (p.tiles_k + (p.db ? 1 : 0));
-    if (p.G > 65535) return fail(BNN_ERR_RANGE, "dW takes up to 65535 members");
-    if (tiles * WN * WK * 64 > 0xffffffffLL) return fail(BNN_ERR_RANGE, "too many tiles for one launch");
+    p.tiles_n = (int32_t)ceil_div(p.N, BT);
+    const int64_t nblk = (int64_t)p.G * ((int64_t)p.tiles_n * p.tiles_k + (p.db ? ceil_div((int64_t)p.N * sizeof(T), STAGE_BYTES) : 0));
+    if (nblk >= (1LL << 32) / (WN * WK * 64)) return fail(BNN_ERR_RANGE, "too many tiles for one launch");
     constexpr auto* kern = &bnn_grouped_dw_kernel<T, T, BT, WN, WK, DMA, LISTED>;
     allow_big_lds<kern>();
-    hipLaunchKernelGGL(*kern, dim3((unsigned)tiles, (unsigned)p.G, (unsigned)p.splits), dim3(WN * WK * 64), (size_t)4 * BT * STAGE_BYTES, st, p);
+    hipLaunchKernelGGL(*kern, dim3((unsigned)nblk, (unsigned)p.splits), dim3(WN * WK * 64), (size_t)4 * BT * STAGE_BYTES, st, p);
     HIP_TRY(hipGetLastError());
     return 0;
 }

@@ -108,5 +108,5 @@ def test_grids_beyond_the_launch_limit_are_refused():
         assert L.bnn_grouped_linear(C.byref(q), 16, 16, None, 16, None) == N.ERR_RANGE
         assert L.bnn_int8_linear(C.byref(q), 16, 16, 16, 16, None, 16, None) == N.ERR_RANGE
     assert L.bnn_grouped_linear_dx(C.byref(grouped(rows=1 << 29, inputs=1 << 24)), 16, 16, 16, None, None) == N.ERR_RANGE
-    assert L.bnn_grouped_linear_dw(C.byref(grouped(members=65536)), 16, 16, 16, None, 16, None) == N.ERR_RANGE
+    assert L.bnn_grouped_linear_dw(C.byref(grouped(members=1 << 24, inputs=1024, outputs=1024)), 16, 16, 16, None, 16, None) == N.ERR_RANGE
     assert L.bnn_grouped_linear_dw(C.byref(grouped(inputs=1 << 24, outputs=1 << 24)), 16, 16, 16, None, 16, None) == N.ERR_RANGE
