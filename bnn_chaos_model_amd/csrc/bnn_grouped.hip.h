@@ -431,23 +431,32 @@ __global__ __launch_bounds__(512) void bnn_grouped_few_kernel(RowsParams p) {
     }
 }
 
-// ---- forward of short rows ----------------------------------------------------------------------------------------------------------------
-// 16 FN outputs of up to 64 ST bytes of reduction: the member's matrix stays in FN x ST fragments of a wave's registers (at most 32: 128
-// registers) while `block_rows` rows of the batch stream by, sixteen at a time and wave by wave -- no LDS, no barrier; what is read and written
-// is the batch.  The rows' places are fetched two steps ahead and the rows one step ahead of their products.
-template <typename T, typename O, int FN, int ST>
+// ---- forward of short rows --------------------------------------------------------------------------------------------------------------
+// Rows of up to 64 ST bytes: the member's matrix stays in registers, FN x ST fragments a wave, while `block_rows` rows of the batch stream by,
+// sixteen at a time -- no LDS, no barrier; what is read and written is the batch.  WN of the four waves share a row (each 16 FN outputs; its second
+// to fourth reading comes from the first-level cache), so that a wave's part of the matrix is small and many waves fit.  The rows' places are
+// fetched two steps ahead and the rows one step ahead of their products.
+template <typename T, typename O, int FN, int ST, int WN>
 __global__ __launch_bounds__(256) void bnn_grouped_short_kernel(RowsParams p) {
-    constexpr int WAVES = 4, BN = 16 * FN, STEP = 64;
+    constexpr int BN = 16 * FN * WN, STEP = 64, MSTEP = 16 * (4 / WN);
     using M = Mma<T>;
     using Acc = typename M::Acc;
     int tm, tn;
     tile_of_block(p.nblk, p.tiles_n, p.band, tm, tn);
     const RowTile rt = find_rows(p.offsets, p.G, p.P, tm, p.block_rows);
     if (rt.g < 0) return;
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n0 = tn * BN, i16 = lane & 15, q = lane >> 4;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n0 = tn * BN + wave % WN * 16 * FN, i16 = lane & 15, q = lane >> 4;
+    if (n0 >= p.N) return;
     const bool nobody = rt.g == p.G && p.offsets;
     const int64_t kbytes = (int64_t)p.K * sizeof(T);
     const char* wg = p.w + (nobody ? 0 : rt.g) * p.w_member;
+    const bool listed = p.gather_div || p.scatter;
+    const auto place = [&](int m) -> int {   // the pair at grouped row m (m itself without an order)
+        const int r = min(m, rt.r1 - 1);
+        return listed ? p.order[r] : r;
+    };
+    int m = rt.r0 + wave / WN * 16 + i16;
+    int pair = place(m), pair1 = place(m + MSTEP);   // (asked for ahead of the matrix: the rows wait for them)
     u32x4 w[FN][ST];
     float bias[FN][4], ws[FN][4];
 #pragma unroll
@@ -464,11 +473,6 @@ __global__ __launch_bounds__(256) void bnn_grouped_short_kernel(RowsParams p) {
             ws[j][i] = sizeof(T) == 1 ? p.ws[col] : 1.0f;
         }
     }
-    const bool listed = p.gather_div || p.scatter;
-    const auto place = [&](int m) -> int {   // the pair at grouped row m (m itself without an order)
-        const int r = min(m, rt.r1 - 1);
-        return listed ? p.order[r] : r;
-    };
     const auto source = [&](int m, int pair) -> int64_t {   // row of x
         if (!p.gather_div) return min(m, rt.r1 - 1);
         const int o = pair >= 0 && pair < p.P ? pair : 0;
@@ -482,15 +486,13 @@ __global__ __launch_bounds__(256) void bnn_grouped_short_kernel(RowsParams p) {
             x[s] = load_chunk<T>(row, at, kbytes, (s + 1) * STEP <= kbytes);
         }
     };
-    int m = rt.r0 + wave * 16 + i16;
-    int pair = place(m), pair1 = place(m + 16 * WAVES);
     int64_t src = source(m, pair);
     u32x4 x[ST];
     if (!nobody) fetch(src, x);
-    for (; m - i16 < rt.r1; m += 16 * WAVES) {
+    for (; m - i16 < rt.r1; m += MSTEP) {
         u32x4 xn[ST];
-        const int64_t src1 = source(m + 16 * WAVES, pair1);
-        const int pair2 = place(m + 32 * WAVES);
+        const int64_t src1 = source(m + MSTEP, pair1);
+        const int pair2 = place(m + 2 * MSTEP);
         if (!nobody) fetch(src1, xn);
         Acc acc[FN];
 #pragma unroll

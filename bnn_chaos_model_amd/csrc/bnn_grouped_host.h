@@ -67,21 +67,18 @@ int launch_few(const RowsParams& p, hipStream_t st) {
 
 template <typename T, typename O, int FN, int ST>
 int launch_rows_short(RowsParams p, hipStream_t st) {
-    // rows per workgroup: as many as let the grid run in whole rounds of two workgroups per CU (320 rows, one round, for 150 000 rows x 128
-    // outputs: 44 us; 256 rows, a fifth more workgroups: 62)
-    const int64_t tiles_n = ceil_div(p.N, 16 * FN), loss = std::min(p.G, p.P) * tiles_n;
-    int64_t room = 512;
-    while (room <= loss) room += 512;
-    p.block_rows = (int32_t)std::max<int64_t>(64, ceil_div(ceil_div(p.P * tiles_n, room - loss / 2), 64) * 64);
-    if (int rc = set_grid(p, p.block_rows, 16 * FN, 1, 256)) return rc;
-    hipLaunchKernelGGL((bnn_grouped_short_kernel<T, O, FN, ST>), dim3((unsigned)p.nblk), dim3(256), 0, st, p);
+    constexpr int WN = 4;
+    // 128 rows per workgroup where that still makes four workgroups per CU (150 000 rows x 41 -> 128: 44 us; 64 rows 47, 256 rows 51), else 64
+    p.block_rows = likely_tiles(p, 128) * ceil_div(p.N, 16 * FN * WN) >= 1024 ? 128 : 64;
+    if (int rc = set_grid(p, p.block_rows, 16 * FN * WN, 1, 256)) return rc;
+    hipLaunchKernelGGL((bnn_grouped_short_kernel<T, O, FN, ST, WN>), dim3((unsigned)p.nblk), dim3(256), 0, st, p);
     HIP_TRY(hipGetLastError());
     return 0;
 }
 
 template <typename T, typename O, int ST>
 int launch_short(const RowsParams& p, hipStream_t st) {
-    return p.N <= 64 ? launch_rows_short<T, O, 4, ST>(p, st) : launch_rows_short<T, O, 8, ST>(p, st);
+    return p.N <= 64 ? launch_rows_short<T, O, 1, ST>(p, st) : launch_rows_short<T, O, 2, ST>(p, st);
 }
 
 // whole, aligned 16-byte chunks along every staged row (and four aligned outputs per store: p.vec)
