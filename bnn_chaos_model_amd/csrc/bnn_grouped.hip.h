@@ -1,6 +1,8 @@
 // bnn_grouped.hip.h -- kernels of the grouped linear layer: the product of ragged row groups with their members' matrices (forward and dX), and
 // the product over the rows of a group (dW, db).  Used by bnn_ops_grouped.hip (float types) and bnn_ops_int8.hip (8-bit operands).
 #pragma once
+#include <type_traits>
+
 #include "bnn_tile.hip.h"
 
 namespace bnn {
@@ -36,6 +38,7 @@ struct ReduceParams {          // dW[g] = sum over rows r of member g of dy_r x_
     int32_t m_x, m_dy;             // -1: row r of the grouped order is row order[r] / copies of x, row order[r] of dy; 0: row r
     uint32_t magic, shift;         // of the division by copies
     int32_t tiles_n, tiles_k, splits;
+    int32_t by_size;               // 1: the members' tiles start in the order of their rows (at most 64 members)
     int32_t vec;                   // K % 4 == 0 and dw aligned to four elements
     __device__ __forceinline__ unsigned by_copies(int pair) const { return __umulhi(2u * (unsigned)pair, magic) >> shift; }
 };
@@ -523,6 +526,22 @@ __global__ __launch_bounds__(256) void bnn_grouped_short_kernel(RowsParams p) {
     }
 }
 
+// the member with the r-th most rows, of up to 64
+__device__ __forceinline__ int largest_member(const int32_t* __restrict__ off, int G, int P, int r) {
+    const int lane = threadIdx.x & 63;
+    int size = -1;
+    if (lane < G) {
+        const int s = min(max(off[lane], 0), P);
+        size = min(max(off[lane + 1], s), P) - s;
+    }
+    int rank = 0;
+    for (int j = 0; j < G; ++j) {
+        const int other = __builtin_amdgcn_readlane(size, j);
+        rank += other > size || (other == size && j < lane) ? 1 : 0;
+    }
+    return __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)__ballot(lane < G && rank == r)) - 1);
+}
+
 // ---- dW, db --------------------------------------------------------------------------------------------------------------------------------
 // BT outputs x BT inputs of one member per workgroup, over split blockIdx.y of the member's rows; further workgroups sum dy's columns, the bias
 // gradient.
@@ -532,22 +551,26 @@ __global__ __launch_bounds__(WN * WK * 64, WN * WK * 64 >= 512 ? 2 : 1) void bnn
     constexpr int NT = WN * WK * 64, FN = BT / WN / 16, FK = BT / WK / 16, BUF = 2 * BT * STAGE_BYTES, KR = stage_k<T>();
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wn = wave / WK, wk = wave % WK;
-    // the workgroups that sum dy's columns come first; behind them XCD x takes the x-th eighth of the tiles, member by member, four output tiles
-    // side by side (what runs together on an XCD shares its operands)
+    // The workgroups that sum dy's columns come first.  Behind them the members' tiles, largest member first (a tile takes as long as its
+    // member has rows; p.by_size), every member spread over all XCDs: XCD x takes the x-th eighth of its tiles, four output tiles side by side, which share their operands
+    // in the XCD's L2.
     constexpr int BC = STAGE_BYTES / (int)sizeof(T);   // dy's columns per workgroup: 128 bytes of a row, for many rows in flight
-    const int ncol = (p.N + BC - 1) / BC, nbias = p.db ? p.G * ncol : 0;
-    const bool bias = (int)blockIdx.x < nbias;
+    const int ncol = (p.N + BC - 1) / BC, nbias = p.db ? p.G * ncol : 0, first = (nbias + 7) / 8 * 8;
+    const bool bias = (int)blockIdx.x < first;
     int g, tn, tk = 0;
     if (bias) {
+        if ((int)blockIdx.x >= nbias) return;
         g = (int)blockIdx.x / ncol;
         tn = (int)blockIdx.x - g * ncol;
     } else {
-        const int all = (int)gridDim.x - nbias, b = (int)blockIdx.x - nbias, per = all / 8, rem = all % 8, x = b % 8;
-        const int i = x * per + min(x, rem) + b / 8, each = p.tiles_n * p.tiles_k;
-        g = i / each;
-        const int in = i - g * each, band = in / (4 * p.tiles_k), at = in - band * 4 * p.tiles_k, rows = min(4, p.tiles_n - band * 4);
+        const int each = p.tiles_n * p.tiles_k, eighth = each < 8 ? 0 : (each + 7) / 8, slots = each < 8 ? each : 8 * eighth, b = (int)blockIdx.x - first;
+        g = b / slots;
+        const int j = b - g * slots, i = each < 8 ? j : (j + g) % 8 * eighth + j / 8;   // (the short last eighth goes round the XCDs)
+        if (i >= each) return;
+        const int band = i / (4 * p.tiles_k), at = i - band * 4 * p.tiles_k, rows = min(4, p.tiles_n - band * 4);
         tk = at / rows;
         tn = band * 4 + at - tk * rows;
+        if (p.by_size) g = largest_member(p.offsets, p.G, p.P, g);
     }
     const int n0 = tn * (bias ? BC : BT), k0 = tk * BT;
     int r0 = min(max(p.offsets[g], 0), p.P), r1 = min(max(p.offsets[g + 1], r0), p.P);
@@ -560,8 +583,8 @@ __global__ __launch_bounds__(WN * WK * 64, WN * WK * 64 >= 512 ? 2 : 1) void bnn
     }
     const bool whole = p.splits == 1;
     const int64_t nk = (int64_t)p.N * p.K, gnk = p.G * nk;
-    if (bias) {   // a thread takes one chunk of every RL-th row, U rows at a time; the RL sums meet in LDS, in order
-        constexpr int E = CHUNK / (int)sizeof(T), CW = BC / E, RL = NT / CW, U = 16;
+    if (bias) {   // a thread takes one chunk of every RL-th row, several at a time; the RL sums meet in LDS, in order
+        constexpr int E = CHUNK / (int)sizeof(T), CW = BC / E, RL = NT / CW;
         float* part = reinterpret_cast<float*>(smem);   // [RL][BC]
         const int c = tid % CW, rl = tid / CW;
         const int64_t width = (int64_t)p.N * sizeof(T), byte = ((int64_t)n0 + c * E) * sizeof(T);
@@ -569,7 +592,8 @@ __global__ __launch_bounds__(WN * WK * 64, WN * WK * 64 >= 512 ? 2 : 1) void bnn
         float s[E];
 #pragma unroll
         for (int e = 0; e < E; ++e) s[e] = 0.0f;
-        for (int r = r0 + rl; r < r1; r += U * RL) {
+        const auto add = [&](int r, auto count) {   // rows r, r + RL, ...
+            constexpr int U = decltype(count)::value;
             int src[U];
             u32x4 v[U];
 #pragma unroll
@@ -592,7 +616,10 @@ __global__ __launch_bounds__(WN * WK * 64, WN * WK * 64 >= 512 ? 2 : 1) void bnn
 #pragma unroll
                 for (int e = 0; e < E; ++e) s[e] += (float)t[e];
             }
-        }
+        };
+        int r = r0 + rl;
+        for (; r + 8 * RL < r1; r += 16 * RL) add(r, std::integral_constant<int, 16>{});
+        for (; r < r1; r += 4 * RL) add(r, std::integral_constant<int, 4>{});
 #pragma unroll
         for (int e = 0; e < E; ++e) part[rl * BC + c * E + e] = s[e];
         __syncthreads();
