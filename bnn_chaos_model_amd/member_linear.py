@@ -163,7 +163,8 @@ def _linear(x, weight, groups, bias, relu, gather, scatter, rows, copies):
 def grouped_linear_grads(dy, x, weight, groups, y=None, gather=False, scatter=False, need=(True, True, True)):
     """Gradients of grouped_linear -> (dx, dweight, dbias), each None where `need` says so.
 
-    dy: gradient of the layer's output, in its shape; y: that output, for a layer with relu=True (the gradient passes where y > 0), else None.
+    dy: gradient of the layer's output, in its shape; y: that output, for a layer with relu=True (no gradient where y <= 0; a NaN output passes it, as in
+    nn.ReLU), else None.
     A plain function without autograd: what grouped_linear's backward calls, and what a captured HIP graph of a training step may call.
     dweight and dbias of a member without rows are zero; sums are fp32 and do not depend on timing."""
     rows, copies = _check_linear(x, weight, groups, None, gather)

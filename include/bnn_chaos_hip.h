@@ -372,7 +372,7 @@ int bnn_multiswag_bands_f32(const bnn_plan* plan, const bnn_grid* grid, const fl
  *   bnn_grouped_linear_dx   dx = W^T dy, the copies of a row added in order (fp32 workspace: bnn_grouped_linear_dx_workspace_bytes)
  *   bnn_grouped_linear_dw   dw [members, outputs, inputs], db [members, outputs] (or NULL), dense; zero for a member without rows.
  *                           The result depends on the shapes only, not on timing: no atomics.
- *   bnn_relu_grad           out[rows, N] (dense) = dy where y > 0, else 0: the gradient in front of the two above for a layer with relu = 1 */
+ *   bnn_relu_grad           out[rows, N] (dense) = 0 where y <= 0, else dy (also where y is NaN): the gradient in front of the two above for a layer with relu = 1 */
 enum bnn_dtype { BNN_TYPE_F32 = 0, BNN_TYPE_BF16 = 1, BNN_TYPE_F16 = 2 };
 typedef struct bnn_grouped {
     int64_t rows;

@@ -273,6 +273,120 @@ def test_infinities_and_nan_stay_in_their_rows(ops):
         assert torch.isnan(ops.grouped_linear(bad, w, gr, bias=b, relu=True, gather=True, scatter=True)[r1]).all()
 
 
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("n,N", [(1, 1), (3, 5), (300, 8), (7, 64), (20000, 136), (20001, 41), (5, 40000), (1100000, 8)])
+def test_relu_mask_of_the_gradient(ops, n, N, dtype):
+    """db of one row a member is the masked dy itself: dense and strided operands, rows on 16-byte borders and not, more chunks than threads in the
+    grid, outputs of zero, minus zero and NaN.  Exact: nothing is rounded."""
+    g = _gen(n + N)
+    y = torch.randint(-2, 3, (n, N), generator=g, device="cuda").to(DT[dtype])
+    dy = torch.randint(1, 9, (n, N), generator=g, device="cuda").to(DT[dtype])
+    y.view(-1)[::7] = -0.0
+    y.view(-1)[::11] = float("nan")
+    want = torch.where(y <= 0, 0.0, dy.float())          # (a comparison with NaN is false: dy passes)
+    wide_y, wide_dy = torch.zeros(n, N + 3, dtype=DT[dtype], device="cuda"), torch.zeros(n, N + 8, dtype=DT[dtype], device="cuda")
+    wide_y[:, 3:], wide_dy[:, :N] = y, dy
+    x = torch.ones(n, 1, dtype=DT[dtype], device="cuda")
+    w = torch.ones(1, N, 1, dtype=DT[dtype], device="cuda")
+    gr = ops.group_rows(torch.zeros(n, dtype=torch.int32, device="cuda"), 1)
+    for yy, dd in ((y, dy), (wide_y[:, 3:], dy), (y, wide_dy[:, :N]), (wide_y[:, 3:], wide_dy[:, :N])):
+        dx, _, db = ops.grouped_linear_grads(dd, x, w, gr, y=yy)
+        rows, cols = want.double().sum(1), want.double().sum(0)   # (sums of positive whole numbers)
+        for got, sums, terms in ((dx[:, 0], rows, N), (db[0], cols, n)):
+            slack = (terms + 2) * 2.0 ** -23 * sums
+            # The largest fp16 number is 65504 and its step there is 32, so that 65520 and more round to infinity: a sum that is certainly beyond
+            # (here 40 000 terms of 1.8 on average) has to be infinite, any other lies within the bound or, next to the border, on either side.
+            top = 65520.0 if got.dtype == torch.float16 else float("inf")
+            assert torch.isinf(got[sums - slack >= top]).all()
+            sure = sums + slack < top
+            within(got[sure], sums[sure], slack[sure])
+
+
+def test_nan_output_passes_the_gradient_as_in_relu(ops):
+    x = torch.tensor([[float("nan")], [1.0], [-1.0], [0.0]], device="cuda", requires_grad=True)
+    w = torch.full((1, 1, 1), 2.0, device="cuda")
+    gr = ops.group_rows(torch.zeros(4, dtype=torch.int32, device="cuda"), 1)
+    y = ops.grouped_linear(x, w, gr, relu=True, gather=True, scatter=True)
+    got, = torch.autograd.grad(y.sum(), x)
+    z = x.detach().clone().requires_grad_(True)
+    want, = torch.autograd.grad(torch.relu(z * 2.0).sum(), z)
+    assert torch.equal(got, want) and float(got[0]) == 2.0
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("n,copies,K", [(1, 2, 1), (3, 3, 5), (4, 2, 8), (2000, 5, 64), (30001, 2, 136), (3001, 3, 41), (2, 4, 20000)])
+def test_copies_of_a_row_add_up(ops, n, copies, K, dtype):
+    """dx of a row is the sum over its copies, those of nobody left out: whole numbers below 256 with one output, so exact in every type."""
+    g = _gen(n + K)
+    m = torch.randint(-1, 3, (n, copies), generator=g, device="cuda", dtype=torch.int32)
+    w = torch.randint(-3, 4, (3, 1, K), generator=g, device="cuda").to(DT[dtype])
+    dy = torch.randint(-4, 5, (n, copies, 1), generator=g, device="cuda").to(DT[dtype])
+    x = torch.zeros(n, K, dtype=DT[dtype], device="cuda")
+    dx, _, _ = ops.grouped_linear_grads(dy, x, w, ops.group_rows(m, 3), gather=True, scatter=True, need=(True, False, False))
+    want = torch.zeros(n, K, device="cuda")
+    for c in range(copies):
+        live = m[:, c] >= 0
+        want[live] += dy[live, c].float() * w[m[live, c].long(), 0].float()
+    assert float(want.abs().max()) <= 60 and torch.equal(dx.float(), want)
+
+
+def test_offsets_beyond_32_bits(ops):
+    """Batches, outputs and weights of more than 2^32 elements: their last rows come out as those rows do alone."""
+    n, K = 131077, 32776
+    assert n * K > 1 << 32
+    x = torch.empty(n, K, dtype=torch.bfloat16, device="cuda").normal_(generator=_gen(1))
+    m = torch.zeros(n, dtype=torch.int32, device="cuda")
+    m[::3] = 1
+    gr = ops.group_rows(m, 2)
+    w = torch.randn(2, 24, K, generator=_gen(2), device="cuda").bfloat16()
+    far = torch.tensor([0, 1, n // 2, n - 3, n - 2, n - 1], device="cuda")
+    xf, mf = x[far].double(), m[far].long()
+
+    def rows_of(a, wm):   # a [6, k] times each row's own matrix [6, n, k]
+        return (wm * a[:, None]).sum(-1), (wm * a[:, None]).abs().sum(-1)
+    y = ops.grouped_linear(x, w, gr, gather=True, scatter=True)
+    want, mag = rows_of(xf, w.double()[mf])
+    within(y[far], want, (K + 2) * 2.0 ** -23 * mag)
+    # dW: only the last three rows have a gradient (products of bf16 are exact in fp32, sums of at most three: two roundings)
+    dy = torch.zeros(n, 24, dtype=torch.bfloat16, device="cuda")
+    dy[far[3:]] = torch.randn(3, 24, generator=_gen(3), device="cuda").bfloat16()
+    dx, dw, _ = ops.grouped_linear_grads(dy, x, w, gr, gather=True, scatter=True)
+    want, mag = rows_of(dy[far].double(), w.double()[mf].transpose(1, 2))
+    within(dx[far], want, 26 * 2.0 ** -23 * mag)
+    for g in (0, 1):
+        pick = far[3:][m[far[3:]] == g]
+        d, a = dy[pick].double(), x[pick].double()
+        within(dw[g], d.t() @ a, 5 * 2.0 ** -23 * (d.abs().t() @ a.abs()))
+    del dx, dw
+    # 8 bits
+    q = ops.quantize_rows(x)
+    near = ops.quantize_rows(x[far])
+    assert torch.equal(q.values[far], near.values) and torch.equal(q.scale[far], near.scale)
+    wq = ops.quantize_rows(w)
+    y8 = ops.int8_linear(q, wq, groups=gr, gather=True, scatter=True)
+    want, mag = rows_of(near.values.double() * near.scale.double()[:, None], wq.values.double()[mf] * wq.scale.double()[mf][..., None])
+    within(y8[far], want, 4 * 2.0 ** -24 * want.abs())   # the integer sum's conversion, the scales' product, theirs
+    del x, q, y, dy
+    # the outputs, and the mask over them
+    a = torch.randn(n, 16, generator=_gen(4), device="cuda").bfloat16()
+    v = torch.randn(2, K, 16, generator=_gen(5), device="cuda").bfloat16()
+    y = ops.grouped_linear(a, v, gr, relu=True, gather=True, scatter=True)
+    want, mag = rows_of(a[far].double(), v.double()[mf])
+    within(y[far], want.clamp_min(0), 18 * 2.0 ** -23 * mag)
+    dy = torch.zeros_like(y)
+    dy[far] = 1.0
+    dx, _, _ = ops.grouped_linear_grads(dy, a, v, gr, y=y, gather=True, scatter=True, need=(True, False, False))
+    want, mag = rows_of((y[far] > 0).double(), v.double()[mf].transpose(1, 2))
+    within(dx[far], want, (K + 2) * 2.0 ** -23 * mag)
+    del y, dy
+    big = torch.empty(3, 40000, 40000, dtype=torch.bfloat16, device="cuda").normal_(generator=_gen(6))
+    assert big.numel() > 1 << 32
+    a = torch.randn(5, 40000, generator=_gen(7), device="cuda").bfloat16()
+    y = ops.grouped_linear(a, big, ops.group_rows(torch.full((5,), 2, dtype=torch.int32, device="cuda"), 3), gather=True, scatter=True)
+    last = big[2, -8:].double()
+    within(y[:, -8:], (a.double()[:, None] * last).sum(-1), 40002 * 2.0 ** -23 * (a.double()[:, None] * last).abs().sum(-1))
+
+
 def test_no_rows(ops):
     m = torch.empty(0, dtype=torch.int32, device="cuda")
     gr = ops.group_rows(m, 3)

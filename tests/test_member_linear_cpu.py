@@ -67,6 +67,9 @@ def test_c_boundary_refuses_missing_pointers_and_sizes():
     assert L.bnn_group_rows_i32(16, 100000, 4, 16, 16, None, None) == N.ERR_INVALID                                    # the sort's workspace
     assert L.bnn_group_rows_i32(16, 4, 4, 16, None, None, None) == N.ERR_INVALID
     assert L.bnn_relu_grad(16, 8, None, 8, 4, 8, 0, 16, None) == N.ERR_INVALID
+    # dx of copies is dense: refused before anything is enqueued
+    assert L.bnn_grouped_linear_dx(C.byref(grouped(copies=2, gather=1, order=16, x_row=9)), 16, 16, 16, 16, None) == N.ERR_INVALID
+    assert b"dense" in L.bnn_last_error()
 
 
 def test_empty_batches_need_no_device():
