@@ -7,6 +7,8 @@
 //   bnn_ops_reduce.hip    predictive moments; predict_instability on an explicit summary
 //   bnn_ops_stats.hip     the evaluation scripts' post-sampling statistics: replay kernels, Philox epilogue, quantile sketch
 //   bnn_ops_features.hip  feature packing + standardisation
+//   bnn_ops_grouped.hip   rows sorted by member; the linear layer over such groups and its gradients
+//   bnn_ops_int8.hip      rows to 8-bit integers; the linear layer on them
 #pragma once
 #include <hip/hip_runtime.h>
 

@@ -12,6 +12,8 @@
 //   bnn_abi.hip         extern "C" entry points that launch a forward kernel, plans, specialised forms (bnn_abi_common.h lists the C-ABI units)
 //   bnn_ops_draw.hip, bnn_ops_reduce.hip, bnn_ops_stats.hip, bnn_ops_features.hip   the small kernels with their entry points: SWAG draw +
 //                       Philox fills; moments + regress_nn on a summary; statistics epilogue + quantile sketch; feature packing
+//   bnn_gmm.hip         products of the linear layer over row groups (bnn_grouped.hip.h; bnn_grouped_host.h chooses)
+//   bnn_ops_grouped.hip, bnn_ops_int8.hip   that layer's entry points, the sort by member, the gradients' sweeps; 8-bit rows and the layer on them
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
