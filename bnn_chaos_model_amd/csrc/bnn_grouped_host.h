@@ -115,7 +115,8 @@ int launch_rows_typed(RowsParams p, hipStream_t st) {
         if (t128 <= t64) return launch_rows_tile<T, O, 128, 128, 2, 2, WFC, true>(p, st);
         return launch_rows_tile<T, O, 64, 64, 2, 2, WFC, true>(p, st);
     }
-    if constexpr (sizeof(T) == 1)   // 16 384 x 4 095 -> 4 096: 542 us against 842 in 128 x 128 tiles
+    // 16 384 x 4 095 -> 4 096 in 8 bits: 542 us against 842 in 128 x 128 tiles (bf16 loses with it: 32 768 x 4 095 -> 4 096 2 250 against 2 000)
+    if constexpr (sizeof(T) == 1)
         if (ceil_div(tiles(256, 128), 256) * 0.41 <= std::min(t128, t64)) return launch_rows_tile<T, O, 256, 128, 4, 2, WFC, false>(p, st);
     if (t128 <= t64) return launch_rows_tile<T, O, 128, 128, 2, 2, WFC, false>(p, st);
     return launch_rows_tile<T, O, 64, 64, 2, 2, WFC, false>(p, st);
