@@ -25,11 +25,6 @@ RowGroups = namedtuple("RowGroups", "order offsets shape")
 QuantRows = namedtuple("QuantRows", "values scale")
 
 
-class _Sorted(RowGroups):
-    """What group_rows returns: its index tensors need no second look at every call."""
-    __slots__ = ()
-
-
 def _gpu(t, name, dtypes):
     if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype not in dtypes:
         got = f"{t.dtype} on {t.device}" if isinstance(t, torch.Tensor) else type(t).__name__
@@ -95,7 +90,7 @@ def group_rows(member, n_members):
     nbytes = 0 if P <= 4096 else N.lib().bnn_group_rows_workspace_bytes(P, n_members)
     ws = m.new_empty(nbytes // 4) if nbytes else None
     _run(m.get_device(), N.lib().bnn_group_rows_i32, m.data_ptr(), P, n_members, order.data_ptr(), offsets.data_ptr(), _addr(ws))
-    return _Sorted(order, offsets, shape)
+    return RowGroups(order, offsets, shape)
 
 
 def _check_groups(groups, x, G, gather, what="x"):
@@ -104,15 +99,23 @@ def _check_groups(groups, x, G, gather, what="x"):
         raise TypeError("groups must be the RowGroups that group_rows returns")
     order, offsets, shape = groups
     dev = x.get_device()
-    rows, copies = shape if len(shape) == 2 else (shape[0], 1)
-    if type(groups) is not _Sorted:
-        _gpu(order, "groups.order", (torch.int32,))
-        _gpu(offsets, "groups.offsets", (torch.int32,))
-        _same_device(dev, "groups.offsets", offsets)
-        if order.numel() != rows * copies or not order.is_contiguous() or not offsets.is_contiguous():
-            raise ValueError("groups.order must be contiguous and hold one entry per (row, copy) pair")
-    if order.get_device() != dev:
-        _same_device(dev, "groups.order", order)
+    if len(shape) == 2:
+        rows, copies = shape
+    elif len(shape) == 1:
+        rows, copies = shape[0], 1
+    else:
+        raise ValueError("groups.shape must be (rows,) or (rows, copies)")
+    try:   # at every call, also of what group_rows made: a named tuple is easily rebuilt around other tensors, and the kernels trust these
+        fit = (order.dtype is torch.int32 and offsets.dtype is torch.int32 and order.get_device() == dev and offsets.get_device() == dev
+               and order.numel() == rows * copies and order.is_contiguous() and offsets.is_contiguous())
+    except AttributeError:
+        fit = False
+    if not fit:
+        for name, t in (("groups.order", order), ("groups.offsets", offsets)):
+            if not isinstance(t, torch.Tensor) or t.dtype is not torch.int32 or t.device.type != x.device.type:
+                raise TypeError(f"{name}: expected a torch.int32 tensor on the rows' device, got " + (f"{t.dtype} on {t.device}" if isinstance(t, torch.Tensor) else type(t).__name__))
+            _same_device(dev, name, t)
+        raise ValueError("groups.order must be contiguous and hold one entry per (row, copy) pair, groups.offsets contiguous")
     if offsets.numel() != G + 1:
         raise ValueError(f"groups are over {offsets.numel() - 1} members, the weights over {G}")
     want = rows if gather else rows * copies
@@ -121,8 +124,8 @@ def _check_groups(groups, x, G, gather, what="x"):
     return rows, copies
 
 
-def _out_shape(groups, n_out, scatter):
-    return (*groups.shape, n_out) if scatter else (groups.order.numel(), n_out)
+def _out_shape(groups, pairs, n_out, scatter):
+    return (*groups.shape, n_out) if scatter else (pairs, n_out)
 
 
 def _check_linear(x, weight, groups, bias, gather):
@@ -154,7 +157,7 @@ def _linear(x, weight, groups, bias, relu, gather, scatter, rows, copies):
     x, weight = _rows2d(x), _layers(weight)
     if bias is not None and not bias.is_contiguous():
         bias = bias.contiguous()
-    y = x.new_empty(_out_shape(groups, weight.shape[1], scatter))
+    y = x.new_empty(_out_shape(groups, rows * copies, weight.shape[1], scatter))
     q = _descriptor(groups, rows, copies, x.dtype, weight, _row_stride(x), weight.shape[1], gather, scatter, relu)
     _run(x.get_device(), N.lib().bnn_grouped_linear, q, x.data_ptr(), weight.data_ptr(), _addr(bias), y.data_ptr())
     return y
@@ -169,7 +172,7 @@ def grouped_linear_grads(dy, x, weight, groups, y=None, gather=False, scatter=Fa
     dweight and dbias of a member without rows are zero; sums are fp32 and do not depend on timing."""
     rows, copies = _check_linear(x, weight, groups, None, gather)
     G, n_out, n_in = weight.shape
-    shape = _out_shape(groups, n_out, scatter)
+    shape = _out_shape(groups, rows * copies, n_out, scatter)
     dev = x.get_device()
     for name, t in (("dy", dy),) if y is None else (("dy", dy), ("y", y)):
         _gpu(t, name, (x.dtype,))
@@ -317,7 +320,7 @@ def int8_linear(x, weight, groups=None, bias=None, relu=False, gather=False, sca
     else:
         rows, copies = _check_groups(groups, rows_of, G, gather)
         order, offsets = groups.order.data_ptr(), groups.offsets.data_ptr()
-        out = _out_shape(groups, n_out, scatter)
+        out = _out_shape(groups, rows * copies, n_out, scatter)
     rows_of, ws = _rows2d(rows_of), ws.contiguous()
     y = rows_of.new_empty(out, dtype=dtype)
     q = N.BnnGrouped(rows, copies, G, n_in, n_out, _TYPES[dtype], 1 if gather else 0, 1 if scatter else 0, 1 if relu else 0, _row_stride(rows_of), n_out,

@@ -1,0 +1,67 @@
+"""CPU: what the linear layers over row groups check before they call a kernel -- groups that a caller has altered, operands whose derivative would be lost."""
+import copy
+
+import pytest
+import torch
+from torch.utils import _pytree
+
+from bnn_chaos_model_amd import member_linear as M
+from bnn_chaos_model_amd import ops
+
+
+# ---- groups --------------------------------------------------------------------------------------------------------------------------------
+def some_groups(rows=6, G=2):
+    return ops.RowGroups(torch.arange(rows, dtype=torch.int32), torch.zeros(G + 1, dtype=torch.int32), (rows,))
+
+
+def check(groups, rows=6, G=2, gather=True):
+    return M._check_groups(groups, torch.zeros(rows, 3), G, gather)   # (both on the CPU: "the same device")
+
+
+def rebuilt(groups, **kw):
+    """The ways a named tuple is made from another one: all of them must end in the same checks."""
+    values = {**groups._asdict(), **kw}
+    yield groups._replace(**kw)
+    yield type(groups)(**values)
+    yield type(groups)._make(values.values())
+    yield copy.copy(groups)._replace(**kw)
+    leaves, spec = _pytree.tree_flatten(groups)
+    yield _pytree.tree_unflatten(leaves, spec)._replace(**kw)
+
+
+def test_groups_as_they_are_made_pass():
+    assert check(some_groups()) == (6, 1)
+    assert check(some_groups()._replace(shape=(3, 2)), rows=3) == (3, 2)
+    assert check(some_groups()._replace(shape=(3, 2)), rows=6, gather=False) == (3, 2)
+
+
+@pytest.mark.parametrize("kw,rows,error", [
+    (dict(shape=(60,)), 60, ValueError),                                       # more pairs than order holds
+    (dict(shape=(6, 7)), 6, ValueError),
+    (dict(shape=(5,)), 5, ValueError),
+    (dict(shape=()), 6, ValueError),
+    (dict(shape=(6, 1, 1)), 6, ValueError),
+    (dict(order=torch.arange(6)), 6, TypeError),                               # 64-bit indices
+    (dict(offsets=torch.zeros(3, dtype=torch.int64)), 6, TypeError),
+    (dict(order=[0, 1, 2, 3, 4, 5]), 6, TypeError),
+    (dict(offsets=None), 6, TypeError),
+    (dict(order=torch.arange(12, dtype=torch.int32)[::2]), 6, ValueError),     # strided
+    (dict(offsets=torch.zeros(6, dtype=torch.int32)[::2]), 6, ValueError),
+    (dict(order=torch.arange(5, dtype=torch.int32)), 6, ValueError),
+    (dict(offsets=torch.zeros(2, dtype=torch.int32)), 6, ValueError)])
+def test_altered_groups_are_refused(kw, rows, error):
+    for groups in rebuilt(some_groups(), **kw):
+        with pytest.raises(error):
+            check(groups, rows=rows)
+
+
+def test_a_tensor_of_the_groups_altered_in_place_is_refused():
+    groups = some_groups()
+    groups.order.resize_(4)
+    with pytest.raises(ValueError):
+        check(groups)
+
+
+def test_group_rows_returns_the_checked_type():
+    """(No subclass that a check could pass over.)"""
+    assert not [c for c in vars(M).values() if isinstance(c, type) and issubclass(c, M.RowGroups) and c is not M.RowGroups]

@@ -1,0 +1,31 @@
+"""GPU: the calls of the linear layers over row groups that their documentation allows and that go wrong easily.
+
+Bounds as in test_member_linear.py: a sum of n products in fp32 is off by at most (n + 1) 2^-23 sum |a b|, and one rounding to the output's type by half a
+step."""
+import numpy as np
+import pytest
+import torch
+
+from test_member_linear import DT, _gen, make, members, ops, pair_view, plain, within  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- altered groups --------------------------------------------------------------------------------------------------------------------------
+def test_altered_groups_are_refused_before_a_launch(ops):
+    m, x, w, b = make(300, 3, 0, 24, 16, torch.float32, True)
+    gr = ops.group_rows(m, 3)
+    wq = ops.quantize_rows(w)
+    dy = torch.ones(300, 16, device="cuda")
+    longer = x.repeat(2, 1)
+    for bad, rows, error in ((gr._replace(shape=(600,)), longer, ValueError), (gr._replace(offsets=gr.offsets.cpu()), x, TypeError), (gr._replace(order=gr.order.cpu()), x, TypeError),
+                             (gr._replace(order=gr.order.long()), x, TypeError), (gr._replace(offsets=gr.offsets.long()), x, TypeError),
+                             (gr._replace(order=gr.order.repeat_interleave(2)[::2]), x, ValueError), (gr._replace(offsets=gr.offsets.repeat_interleave(2)[::2]), x, ValueError)):
+        with pytest.raises(error):
+            ops.grouped_linear(rows, w, bad, bias=b, gather=True, scatter=True)
+        with pytest.raises(error):
+            ops.grouped_linear_grads(dy, rows, w, bad, gather=True, scatter=True)
+        with pytest.raises(error):
+            ops.int8_linear(rows, wq, groups=bad, bias=b, gather=True, scatter=True)
+    same = gr._replace(shape=(300, 1))
+    assert torch.equal(ops.grouped_linear(x, w, same, bias=b, gather=True, scatter=True)[:, 0], ops.grouped_linear(x, w, gr, bias=b, gather=True, scatter=True))
