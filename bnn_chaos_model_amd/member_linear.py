@@ -9,6 +9,7 @@ import ctypes as C
 from collections import namedtuple
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _native as N
@@ -35,6 +36,13 @@ def _gpu(t, name, dtypes):
 def _same_device(dev, name, t):
     if t.get_device() != dev:
         raise ValueError(f"{name} is on {t.device}, the rows are on cuda:{dev}")
+
+
+def _no_tangents(**operands):
+    """Refuse operands of forward-mode differentiation (a native call reads the values alone: the derivative would come out as zero)."""
+    for name, t in operands.items():
+        if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"{name} carries a forward-mode tangent: these layers have no forward-mode derivative")
 
 
 def _run(dev, fn, *args):
@@ -129,6 +137,8 @@ def _out_shape(groups, pairs, n_out, scatter):
 
 
 def _check_linear(x, weight, groups, bias, gather):
+    if forward_ad._current_level >= 0:   # (inside a dual_level; outside of one there are no tangents)
+        _no_tangents(x=x, weight=weight, bias=bias)
     _gpu(x, "x", _FLOATS)
     dtype, dev = x.dtype, x.get_device()
     _gpu(weight, "weight", (dtype,))
@@ -170,6 +180,8 @@ def grouped_linear_grads(dy, x, weight, groups, y=None, gather=False, scatter=Fa
     nn.ReLU), else None.
     A plain function without autograd: what grouped_linear's backward calls, and what a captured HIP graph of a training step may call.
     dweight and dbias of a member without rows are zero; sums are fp32 and do not depend on timing."""
+    if forward_ad._current_level >= 0:
+        _no_tangents(dy=dy, y=y)
     rows, copies = _check_linear(x, weight, groups, None, gather)
     G, n_out, n_in = weight.shape
     shape = _out_shape(groups, rows * copies, n_out, scatter)
@@ -242,6 +254,8 @@ def grouped_linear(x, weight, groups, bias=None, relu=False, gather=False, scatt
 
 
 def _check_quantize(x):
+    if forward_ad._current_level >= 0:
+        _no_tangents(x=x)
     _gpu(x, "x", _FLOATS)
     K = x.shape[-1] if x.dim() else 0
     if K < 1:
@@ -273,6 +287,11 @@ def int8_linear(x, weight, groups=None, bias=None, relu=False, gather=False, sca
     [members, N, K] with groups / gather / scatter as in grouped_linear.  bias [N] or [members, N] in the output's type `dtype` (default: x's
     type; float32 for QuantRows).  Inference only; K <= 131072."""
     quant = isinstance(x, QuantRows)
+    if forward_ad._current_level >= 0:
+        for name, t in (("x", x), ("weight", weight)):
+            if isinstance(t, QuantRows):
+                _no_tangents(**{f"{name}.scale": t.scale})
+        _no_tangents(bias=bias)
     if quant:
         rows_of, xs = _gpu(x.values, "x.values", (torch.int8,)), _gpu(x.scale, "x.scale", (torch.float32,))
     else:

@@ -3,6 +3,7 @@ import copy
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 from torch.utils import _pytree
 
 from bnn_chaos_model_amd import member_linear as M
@@ -65,3 +66,36 @@ def test_a_tensor_of_the_groups_altered_in_place_is_refused():
 def test_group_rows_returns_the_checked_type():
     """(No subclass that a check could pass over.)"""
     assert not [c for c in vars(M).values() if isinstance(c, type) and issubclass(c, M.RowGroups) and c is not M.RowGroups]
+
+
+# ---- forward-mode derivatives ----------------------------------------------------------------------------------------------------------------
+def layer_calls():
+    """(name of the operand that is replaced, the call with it) of every entry point that takes values a derivative may run through."""
+    x, w, b, dy = torch.zeros(6, 3), torch.zeros(2, 4, 3), torch.zeros(2, 4), torch.zeros(6, 4)
+    gr = some_groups()
+    xq, wq = ops.QuantRows(torch.zeros(6, 3, dtype=torch.int8), torch.ones(6)), ops.QuantRows(torch.zeros(2, 4, 3, dtype=torch.int8), torch.ones(2, 4))
+    yield "x", x, lambda t: ops.grouped_linear(t, w, gr, bias=b)
+    yield "weight", w, lambda t: ops.grouped_linear(x, t, gr, bias=b)
+    yield "bias", b, lambda t: ops.grouped_linear(x, w, gr, bias=t)
+    yield "dy", dy, lambda t: ops.grouped_linear_grads(t, x, w, gr)
+    yield "x", x, lambda t: ops.grouped_linear_grads(dy, t, w, gr)
+    yield "weight", w, lambda t: ops.grouped_linear_grads(dy, x, t, gr)
+    yield "y", dy, lambda t: ops.grouped_linear_grads(dy, x, w, gr, y=t)
+    yield "x", x, lambda t: ops.quantize_rows(t)
+    yield "x", x, lambda t: ops.int8_linear(t, wq, groups=gr)
+    yield "bias", b, lambda t: ops.int8_linear(x, wq, groups=gr, bias=t)
+    yield "x.scale", xq.scale, lambda t: ops.int8_linear(xq._replace(scale=t), wq, groups=gr)
+    yield "weight.scale", wq.scale, lambda t: ops.int8_linear(xq, wq._replace(scale=t), groups=gr)
+
+
+@pytest.mark.parametrize("i", range(12))
+def test_operands_with_a_tangent_are_refused(i):
+    """... instead of a result without one, which a caller reads as a derivative of zero."""
+    name, t, call = list(layer_calls())[i]
+    with forward_ad.dual_level():
+        with pytest.raises(NotImplementedError, match=f"^{name} carries a forward-mode tangent"):
+            call(forward_ad.make_dual(t, torch.ones_like(t)))
+        with torch.no_grad(), pytest.raises(NotImplementedError):
+            call(forward_ad.make_dual(t, torch.ones_like(t)))
+        with pytest.raises(TypeError):       # a plain operand next to a dual level: the next check (these are on the CPU)
+            call(t)

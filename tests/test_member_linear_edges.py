@@ -29,3 +29,24 @@ def test_altered_groups_are_refused_before_a_launch(ops):
             ops.int8_linear(rows, wq, groups=bad, bias=b, gather=True, scatter=True)
     same = gr._replace(shape=(300, 1))
     assert torch.equal(ops.grouped_linear(x, w, same, bias=b, gather=True, scatter=True)[:, 0], ops.grouped_linear(x, w, gr, bias=b, gather=True, scatter=True))
+
+
+# ---- forward-mode derivatives ------------------------------------------------------------------------------------------------------------------
+def test_operands_with_a_tangent_are_refused(ops):
+    from torch.autograd import forward_ad
+    m, x, w, b = make(300, 3, 0, 24, 16, torch.float32, True)
+    gr = ops.group_rows(m, 3)
+    want = ops.grouped_linear(x, w, gr, bias=b, gather=True, scatter=True)
+    with forward_ad.dual_level():
+        for i in range(3):
+            for grad in (False, True):       # a dual tensor requires no gradient by itself
+                t = [a.clone() for a in (x, w, b)]
+                t[i] = forward_ad.make_dual(t[i].requires_grad_(grad), torch.ones_like(t[i]))
+                with pytest.raises(NotImplementedError):
+                    ops.grouped_linear(t[0], t[1], gr, bias=t[2], gather=True, scatter=True)
+        leaf = x.clone().requires_grad_(True)
+        y = ops.grouped_linear(leaf, w, gr, bias=b, gather=True, scatter=True)
+        with pytest.raises(NotImplementedError):   # forward over reverse
+            torch.autograd.grad(y, leaf, forward_ad.make_dual(torch.ones_like(y), torch.ones_like(y)))
+        assert torch.equal(ops.grouped_linear(x, w, gr, bias=b, gather=True, scatter=True), want)
+    assert torch.equal(ops.grouped_linear(x, w, gr, bias=b, gather=True, scatter=True), want)
