@@ -285,7 +285,7 @@ def int8_linear(x, weight, groups=None, bias=None, relu=False, gather=False, sca
 
     x [rows, K]: float rows (quantised here: quantize_rows) or QuantRows made earlier; weight: QuantRows of [N, K] (one matrix; groups=None) or of
     [members, N, K] with groups / gather / scatter as in grouped_linear.  bias [N] or [members, N] in the output's type `dtype` (default: x's
-    type; float32 for QuantRows).  Inference only; K <= 131072."""
+    type; float32 for QuantRows).  Inference only: operands that require a gradient are refused under grad mode.  K <= 131072."""
     quant = isinstance(x, QuantRows)
     if forward_ad._current_level >= 0:
         for name, t in (("x", x), ("weight", weight)):
@@ -316,6 +316,8 @@ def int8_linear(x, weight, groups=None, bias=None, relu=False, gather=False, sca
         raise ValueError(f"K must not exceed {_INT8_MAX_INPUTS}: the sums are 32-bit integers")
     if G > 1 << 24 or n_out > 1 << 24:
         raise ValueError("members and outputs must stay below 2^24")
+    if torch.is_grad_enabled() and (ws.requires_grad or (quant and xs.requires_grad)):
+        raise NotImplementedError(f"the 8-bit layer has no gradient: detach {'weight' if ws.requires_grad else 'x'}.scale")
     if ws.shape != shape[:-1] or (quant and xs.shape != rows_of.shape[:1]):
         raise ValueError("scales must have their values' shape without the last dimension")
     dev = rows_of.get_device()

@@ -50,3 +50,19 @@ def test_operands_with_a_tangent_are_refused(ops):
             torch.autograd.grad(y, leaf, forward_ad.make_dual(torch.ones_like(y), torch.ones_like(y)))
         assert torch.equal(ops.grouped_linear(x, w, gr, bias=b, gather=True, scatter=True), want)
     assert torch.equal(ops.grouped_linear(x, w, gr, bias=b, gather=True, scatter=True), want)
+
+
+# ---- 8 bits: no gradient is lost -----------------------------------------------------------------------------------------------------------------
+def test_8_bit_operands_that_require_a_gradient_are_refused(ops):
+    m, x, w, b = make(40, 3, 0, 24, 16, torch.float32, True)
+    gr, xq, wq = ops.group_rows(m, 3), ops.quantize_rows(x), ops.quantize_rows(w)
+    f = lambda xx, ww, bb: ops.int8_linear(xx, ww, groups=gr, bias=bb, gather=True, scatter=True)
+    leaf = lambda t: t.clone().requires_grad_(True)
+    for args in ((xq._replace(scale=leaf(xq.scale)), wq, b), (xq, wq._replace(scale=leaf(wq.scale)), b), (x, wq._replace(scale=leaf(wq.scale)), b), (leaf(x), wq, b), (xq, wq, leaf(b))):
+        with pytest.raises(NotImplementedError, match="no gradient"):
+            f(*args)
+        with torch.no_grad():
+            assert torch.equal(f(*args), f(xq, wq, b))
+    dense = ops.QuantRows(wq.values[0], leaf(wq.scale[0]))
+    with pytest.raises(NotImplementedError, match="weight.scale"):
+        ops.int8_linear(x, dense)
