@@ -322,7 +322,7 @@ __device__ __forceinline__ void grouped_tile(const RowsParams& p, const RowTile 
             float v[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                v[i] = (sizeof(T) == 1 ? (float)acc[j][f][i] * (xs * ws[j][i]) : (float)acc[j][f][i]) + bias[j][i];
+                v[i] = (sizeof(T) == 1 ? sum_f32(acc[j][f][i]) * (xs * ws[j][i]) : sum_f32(acc[j][f][i])) + bias[j][i];
                 if (p.relu) v[i] = v[i] < 0.0f ? 0.0f : v[i];   // (NaN stays NaN, as in nn.ReLU)
             }
             store4<O>(row, n0 + wn * (BN / WN) + j * 16 + (lane >> 4) * 4, p.N, v, DMA || p.vec);
@@ -411,7 +411,7 @@ __global__ __launch_bounds__(512) void bnn_grouped_few_kernel(RowsParams p) {
     __syncthreads();
     for (int t = tid; t < FM * FN * 64; t += 512) {
         Acc a = part[t];
-        for (int w = 1; w < WAVES; ++w) a += part[w * FM * FN * 64 + t];
+        for (int w = 1; w < WAVES; ++w) a = join(a, part[w * FM * FN * 64 + t]);
         const int frag = t >> 6, l = t & 63;
         const int m = rt.r0 + frag / FN * 16 + (l & 15), n = n0 + frag % FN * 16 + (l >> 4) * 4;
         if (m >= rt.r1) continue;
@@ -428,7 +428,7 @@ __global__ __launch_bounds__(512) void bnn_grouped_few_kernel(RowsParams p) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int64_t col = (int64_t)rt.g * p.N + min(n + i, p.N - 1);
-                v[i] = sizeof(T) == 1 ? (float)a[i] * (xs * p.ws[col]) : (float)a[i];
+                v[i] = sizeof(T) == 1 ? sum_f32(a[i]) * (xs * p.ws[col]) : sum_f32(a[i]);
                 if (p.bias) v[i] += (float)reinterpret_cast<const O*>(p.bias)[col];
                 if (p.relu) v[i] = v[i] < 0.0f ? 0.0f : v[i];
             }

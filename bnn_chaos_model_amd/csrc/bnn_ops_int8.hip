@@ -281,7 +281,7 @@ int check_int8(const bnn_grouped* q) {
     if (q->rows < 0 || q->copies < 1 || q->members < 1 || q->inputs < 1 || q->outputs < 1) return fail(BNN_ERR_INVALID, "bad rows / copies / members / inputs / outputs");
     if (q->rows >= (1LL << 30) / q->copies + ((1LL << 30) % q->copies != 0)) return fail(BNN_ERR_RANGE, "rows x copies must stay below 2^30");
     if (q->outputs > (1 << 24) || q->members > (1 << 24)) return fail(BNN_ERR_RANGE, "members and outputs must stay below 2^24");
-    if (q->inputs > 131072) return fail(BNN_ERR_RANGE, "the 32-bit sums hold up to 131072 products of 8-bit integers");   // 2^17 * 127^2 < 2^31
+    if (q->inputs > 131072) return fail(BNN_ERR_RANGE, "the 32-bit sums hold up to 131072 products of 8-bit integers");   // 2^17 * 128^2 = 2^31: sum_f32
     if (q->rows == 0) return 0;
     if ((q->gather || q->scatter) && !q->order) return fail(BNN_ERR_INVALID, "gather / scatter need order");
     if (!q->offsets && (q->members != 1 || q->copies != 1 || q->gather || q->scatter)) return fail(BNN_ERR_INVALID, "without offsets there is one member and no order");

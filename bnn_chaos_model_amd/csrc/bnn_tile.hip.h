@@ -62,6 +62,13 @@ template <> struct Mma<int8_t> {
     }
 };
 
+// Partial sums joined.  Whole numbers as unsigned ones: 2^17 products of -128 and -128 are 2^31, the one sum beyond 32 signed bits (the least is
+// -2^17 x 128 x 127), and it stands as the lowest value until it becomes a float.
+__device__ __forceinline__ tf32x4 join(tf32x4 a, tf32x4 b) { return a + b; }
+__device__ __forceinline__ i32x4 join(i32x4 a, i32x4 b) { return __builtin_bit_cast(i32x4, __builtin_bit_cast(u32x4, a) + __builtin_bit_cast(u32x4, b)); }
+__device__ __forceinline__ float sum_f32(float s) { return s; }
+__device__ __forceinline__ float sum_f32(int32_t s) { return s == INT32_MIN ? 0x1p31f : (float)s; }
+
 // ---- 16-byte loads of rows with any alignment and any length -------------------------------------------------------------------------
 struct __attribute__((packed, aligned(1))) Bytes16 { u32x4 v; };
 __device__ __forceinline__ u32x4 load_any(const char* at) { return reinterpret_cast<const Bytes16*>(at)->v; }

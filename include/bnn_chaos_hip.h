@@ -394,7 +394,7 @@ int bnn_relu_grad(const void* dy, int64_t dy_row, const void* y, int64_t y_row, 
  * not that of a rounded reciprocal.  A row of zeros has scale 0; a row that holds NaN or +-inf has scale NaN and codes 0, so that everything
  * computed from it is NaN.  q rows are q_row >= K bytes apart and zero behind K.
  * bnn_int8_linear: y(r, n) = act(sum_k q(r, k) w(m, n, k) * (x_scale[row] * w_scale[m, n]) + bias[m, n]); integer sums are exact (inputs <=
- * 131072).  q->dtype is the type of bias and y.  offsets = NULL: a dense layer (members = copies = 1). */
+ * 131072, any codes).  q->dtype is the type of bias and y.  offsets = NULL: a dense layer (members = copies = 1). */
 int bnn_quantize_rows(const void* x, int32_t dtype, int64_t rows, int32_t K, int64_t x_row, int8_t* q, int64_t q_row, float* scale, void* stream);
 int bnn_int8_linear(const bnn_grouped* q, const int8_t* x, const float* x_scale, const int8_t* w, const float* w_scale, const void* bias, void* y,
                     void* stream);

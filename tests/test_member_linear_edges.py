@@ -66,3 +66,20 @@ def test_8_bit_operands_that_require_a_gradient_are_refused(ops):
     dense = ops.QuantRows(wq.values[0], leaf(wq.scale[0]))
     with pytest.raises(NotImplementedError, match="weight.scale"):
         ops.int8_linear(x, dense)
+
+
+# ---- 8 bits: the largest sum -----------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("K", [131072, 131071, 131056, 131057])
+@pytest.mark.parametrize("n,N", [(3, 20), (3, 600), (200, 40), (200, 2048), (1100, 2050)])
+def test_sums_of_the_lowest_code(ops, n, N, K):
+    """Codes that a caller brings may be -128, which quantize_rows never gives: 2^17 products of two of them are 2^31.  Exact: a sum is
+    rounded once, to a float32."""
+    one = lambda k: torch.ones(k, device="cuda")
+    q = torch.full((n, K), -128, dtype=torch.int8, device="cuda")
+    w = torch.full((N, K), -128, dtype=torch.int8, device="cuda")
+    w[N // 2:] = 127
+    q[n // 2:] = 127
+    y = ops.int8_linear(ops.QuantRows(q, one(n)), ops.QuantRows(w, one(N)))
+    f = lambda a, b: float(np.float32(a * b * K))
+    assert (y[:n // 2, :N // 2] == f(-128, -128)).all() and (y[:n // 2, N // 2:] == f(-128, 127)).all()
+    assert (y[n // 2:, :N // 2] == f(127, -128)).all() and (y[n // 2:, N // 2:] == f(127, 127)).all()
