@@ -477,7 +477,7 @@ __global__ __launch_bounds__(256) void bnn_grouped_short_kernel(RowsParams p) {
         for (int i = 0; i < 4; ++i) {
             const int64_t col = (int64_t)(nobody ? 0 : rt.g) * p.N + min(n0 + j * 16 + q * 4 + i, p.N - 1);
             bias[j][i] = p.bias && !nobody ? (float)reinterpret_cast<const O*>(p.bias)[col] : 0.0f;
-            ws[j][i] = sizeof(T) == 1 ? p.ws[col] : 1.0f;
+            ws[j][i] = sizeof(T) == 1 && !nobody ? p.ws[col] : 1.0f;   // (nobody's sums are zero, but zero times a NaN scale is not)
         }
     }
     const auto source = [&](int m, int pair) -> int64_t {   // row of x

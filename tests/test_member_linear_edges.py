@@ -83,3 +83,22 @@ def test_sums_of_the_lowest_code(ops, n, N, K):
     f = lambda a, b: float(np.float32(a * b * K))
     assert (y[:n // 2, :N // 2] == f(-128, -128)).all() and (y[:n // 2, N // 2:] == f(-128, 127)).all()
     assert (y[n // 2:, :N // 2] == f(127, -128)).all() and (y[n // 2:, N // 2:] == f(127, 127)).all()
+
+
+# ---- 8 bits: rows of nobody ------------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("n,G,K,N", [(20, 3, 41, 40), (40, 1, 4096, 80), (300, 3, 256, 64), (3000, 9, 41, 40), (3000, 9, 61, 130), (4000, 2, 255, 200), (3000, 3, 511, 96), (700, 3, 2048, 2048)])
+def test_rows_of_nobody_are_zero_next_to_weights_that_are_not_finite(ops, n, G, K, N):
+    """A NaN in a channel of any member's matrix makes that output of the member's own rows NaN, and nothing else."""
+    m, x, w, b = make(n, G, 0, K, N, torch.float32, True, seed=n + K)
+    m[::7] = -1
+    gr = ops.group_rows(m, G)
+    clean = ops.int8_linear(x, ops.quantize_rows(w), groups=gr, bias=b, gather=True, scatter=True)
+    for g in (0, G - 1):
+        bad = w.clone()
+        bad[g, ::5, 3] = float("nan")
+        for relu in (False, True):
+            y = ops.int8_linear(x, ops.quantize_rows(bad), groups=gr, bias=b, relu=relu, gather=True, scatter=True)
+            want = clean.clamp_min(0) if relu else clean.clone()
+            want[(m == g)[:, None] & (torch.arange(N, device="cuda") % 5 == 0)] = float("nan")
+            assert torch.equal(torch.isnan(y), torch.isnan(want)) and torch.equal(y.nan_to_num(7.0), want.nan_to_num(7.0))
+            assert (y[m < 0] == 0).all()
