@@ -288,14 +288,15 @@ __device__ __forceinline__ void grouped_tile(const RowsParams& p, const RowTile 
         else if constexpr (WFC) fb[i - FM] = frag_fc<T, BN>(b, wn * (BN / WN) + (i - FM) * 16, st, lane);
         else fb[i - FM] = frag_kc<T>(b, wn * (BN / WN) + (i - FM) * 16, st, lane);
     });
-    tf32x4 bias[FN], ws[FN];   // of this lane's four outputs per fragment (outputs behind N: not stored)
+    tf32x4 bias[FN];   // of this lane's four outputs per fragment (outputs behind N: not stored)
+    Scale ws[FN][4];
 #pragma unroll
     for (int j = 0; j < FN; ++j)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int64_t col = (int64_t)rt.g * p.N + min(n0 + wn * (BN / WN) + j * 16 + (lane >> 4) * 4 + i, p.N - 1);
             bias[j][i] = 0.0f;
-            ws[j][i] = sizeof(T) == 1 ? p.ws[col] : 1.0f;
+            if constexpr (sizeof(T) == 1) ws[j][i] = Scale(p.ws[col]);
         }
     if (p.bias)
 #pragma unroll
@@ -308,21 +309,21 @@ __device__ __forceinline__ void grouped_tile(const RowsParams& p, const RowTile 
         const int m = rt.r0 + wm * (BM / WM) + f * 16 + (lane & 15);
         char* row = out_row(m);
         if (!row) continue;
-        float xs = 1.0f;
+        Scale xs;
         if constexpr (sizeof(T) == 1) {
             int64_t src = m;
             if (p.gather_div) {
                 const int o = p.order[m];
                 src = o >= 0 && o < p.P ? o / p.gather_div : 0;
             }
-            xs = p.xs[src];
+            xs = Scale(p.xs[src]);
         }
 #pragma unroll
         for (int j = 0; j < FN; ++j) {
             float v[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                v[i] = (sizeof(T) == 1 ? sum_f32(acc[j][f][i]) * (xs * ws[j][i]) : sum_f32(acc[j][f][i])) + bias[j][i];
+                v[i] = value_of(acc[j][f][i], xs, ws[j][i]) + bias[j][i];
                 if (p.relu) v[i] = v[i] < 0.0f ? 0.0f : v[i];   // (NaN stays NaN, as in nn.ReLU)
             }
             store4<O>(row, n0 + wn * (BN / WN) + j * 16 + (lane >> 4) * 4, p.N, v, DMA || p.vec);
@@ -424,11 +425,13 @@ __global__ __launch_bounds__(512) void bnn_grouped_few_kernel(RowsParams p) {
         }
         float v[4] = {0, 0, 0, 0};
         if (!nobody) {
-            const float xs = sizeof(T) == 1 ? p.xs[src] : 1.0f;
+            Scale xs, ws;
+            if constexpr (sizeof(T) == 1) xs = Scale(p.xs[src]);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int64_t col = (int64_t)rt.g * p.N + min(n + i, p.N - 1);
-                v[i] = sizeof(T) == 1 ? sum_f32(a[i]) * (xs * p.ws[col]) : sum_f32(a[i]);
+                if constexpr (sizeof(T) == 1) ws = Scale(p.ws[col]);
+                v[i] = value_of(a[i], xs, ws);
                 if (p.bias) v[i] += (float)reinterpret_cast<const O*>(p.bias)[col];
                 if (p.relu) v[i] = v[i] < 0.0f ? 0.0f : v[i];
             }
@@ -465,7 +468,8 @@ __global__ __launch_bounds__(256) void bnn_grouped_short_kernel(RowsParams p) {
     int m = rt.r0 + wave / WN * 16 + i16;
     int pair = place(m), pair1 = place(m + MSTEP);   // (asked for ahead of the matrix: the rows wait for them)
     u32x4 w[FN][ST];
-    float bias[FN][4], ws[FN][4];
+    float bias[FN][4];
+    Scale ws[FN][4];
 #pragma unroll
     for (int j = 0; j < FN; ++j) {
 #pragma unroll
@@ -477,7 +481,7 @@ __global__ __launch_bounds__(256) void bnn_grouped_short_kernel(RowsParams p) {
         for (int i = 0; i < 4; ++i) {
             const int64_t col = (int64_t)(nobody ? 0 : rt.g) * p.N + min(n0 + j * 16 + q * 4 + i, p.N - 1);
             bias[j][i] = p.bias && !nobody ? (float)reinterpret_cast<const O*>(p.bias)[col] : 0.0f;
-            ws[j][i] = sizeof(T) == 1 && !nobody ? p.ws[col] : 1.0f;   // (nobody's sums are zero, but zero times a NaN scale is not)
+            if constexpr (sizeof(T) == 1) ws[j][i] = Scale(nobody ? 1.0f : p.ws[col]);   // (nobody's sums are zero, but zero times a NaN scale is not)
         }
     }
     const auto source = [&](int m, int pair) -> int64_t {   // row of x
@@ -512,13 +516,14 @@ __global__ __launch_bounds__(256) void bnn_grouped_short_kernel(RowsParams p) {
         const int o = p.scatter ? pair : m;
         if (m < rt.r1 && o >= 0 && o < p.P) {
             char* row = p.y + (int64_t)o * p.ldy;
-            const float xs = sizeof(T) == 1 && !nobody ? p.xs[src] : 1.0f;
+            Scale xs;
+            if constexpr (sizeof(T) == 1) xs = Scale(nobody ? 1.0f : p.xs[src]);
 #pragma unroll
             for (int j = 0; j < FN; ++j) {
                 float v[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    v[i] = (sizeof(T) == 1 ? (float)acc[j][i] * (xs * ws[j][i]) : (float)acc[j][i]) + bias[j][i];
+                    v[i] = value_of(acc[j][i], xs, ws[j][i]) + bias[j][i];
                     if (p.relu) v[i] = v[i] < 0.0f ? 0.0f : v[i];
                 }
                 store4<O>(row, n0 + j * 16 + q * 4, p.N, v, p.vec);

@@ -251,7 +251,7 @@ __global__ __launch_bounds__(512) void bnn_int8_handful_kernel(RowsParams p, int
     __syncthreads();
     if (tid >= 64) return;
     i32x4 a = part[lane];
-    for (int w = 1; w < WAVES; ++w) a += part[w * 64 + lane];
+    for (int w = 1; w < WAVES; ++w) a = join(a, part[w * 64 + lane]);
     const int m = rt.r0 + i16, n = n0 + (lane >> 4) * 4;
     if (m >= rt.r1) return;
     int64_t o = m;
@@ -264,7 +264,7 @@ __global__ __launch_bounds__(512) void bnn_int8_handful_kernel(RowsParams p, int
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int64_t col = (int64_t)rt.g * p.N + min(n + i, p.N - 1);
-            v[i] = (float)a[i] * (sx[i16] * p.ws[col]);
+            v[i] = value_of(a[i], Scale(sx[i16]), Scale(p.ws[col]));
             if (p.bias) v[i] += (float)reinterpret_cast<const O*>(p.bias)[col];
             if (p.relu) v[i] = v[i] < 0.0f ? 0.0f : v[i];
         }

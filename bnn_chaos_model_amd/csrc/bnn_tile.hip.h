@@ -66,8 +66,19 @@ template <> struct Mma<int8_t> {
 // -2^17 x 128 x 127), and it stands as the lowest value until it becomes a float.
 __device__ __forceinline__ tf32x4 join(tf32x4 a, tf32x4 b) { return a + b; }
 __device__ __forceinline__ i32x4 join(i32x4 a, i32x4 b) { return __builtin_bit_cast(i32x4, __builtin_bit_cast(u32x4, a) + __builtin_bit_cast(u32x4, b)); }
-__device__ __forceinline__ float sum_f32(float s) { return s; }
 __device__ __forceinline__ float sum_f32(int32_t s) { return s == INT32_MIN ? 0x1p31f : (float)s; }
+
+// What a product's sum stands for.  Of 8-bit operands: sum * (xs * ws), the scales taken apart into mantissa and exponent, so that their product may be
+// far smaller or larger than a float (1e-30 and 1e-20; 1e30 and 1e30 where the sum is zero).  Where every
+// factor and product is a normal float the bits are those of the plain product.
+struct Scale {
+    float m;   // in [0.5, 1); zero, NaN and infinity stay as they are
+    int e;
+    __device__ __forceinline__ Scale() : m(1.0f), e(0) {}
+    __device__ __forceinline__ explicit Scale(float s) : m(__builtin_amdgcn_frexp_mantf(s)), e(__builtin_amdgcn_frexp_expf(s)) {}
+};
+__device__ __forceinline__ float value_of(int32_t sum, Scale xs, Scale ws) { return __builtin_amdgcn_ldexpf(sum_f32(sum) * (xs.m * ws.m), xs.e + ws.e); }
+__device__ __forceinline__ float value_of(float sum, Scale, Scale) { return sum; }
 
 // ---- 16-byte loads of rows with any alignment and any length -------------------------------------------------------------------------
 struct __attribute__((packed, aligned(1))) Bytes16 { u32x4 v; };

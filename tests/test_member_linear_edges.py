@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 import torch
 
-from test_member_linear import DT, _gen, make, members, ops, pair_view, plain, within  # noqa: F401
+from test_member_linear import DT, INT8_SLACK, _gen, int8_plain, make, members, ops, pair_view, plain, within  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -102,3 +102,34 @@ def test_rows_of_nobody_are_zero_next_to_weights_that_are_not_finite(ops, n, G, 
             want[(m == g)[:, None] & (torch.arange(N, device="cuda") % 5 == 0)] = float("nan")
             assert torch.equal(torch.isnan(y), torch.isnan(want)) and torch.equal(y.nan_to_num(7.0), want.nan_to_num(7.0))
             assert (y[m < 0] == 0).all()
+
+
+# ---- 8 bits: scales whose product no float holds -----------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("n,K,N", [(3, 4096, 20), (20, 200, 600), (3000, 41, 40), (3000, 201, 130), (300, 512, 64), (3000, 640, 384), (3001, 641, 383), (16384, 512, 4096), (16384, 513, 4095)])
+@pytest.mark.parametrize("a,b", [(-22, -20), (-40, -4), (-20, -24), (30, 9), (5, 34), (38, -38), (-44, 30)])
+def test_scales_whose_product_no_float_holds(ops, n, K, N, a, b):
+    """The sum times the scales in 64 bits: where it is a float, the output is that float to four roundings (and half the smallest subnormal) although the
+    scales' product under- or overflows; a sum of zero is zero, a result beyond the floats infinite.  Ready codes, and (rows of few inputs and many) float rows."""
+    g = _gen(n + K)
+    q = torch.randint(-127, 128, (n, K), generator=g, device="cuda", dtype=torch.int8)
+    w = torch.randint(-127, 128, (N, K), generator=g, device="cuda", dtype=torch.int8)
+    q[::5] = 0                                    # sums of zero
+    w[::7] = 0
+    s = (0.5 + torch.rand(n, generator=g, device="cuda", dtype=torch.float64)).mul(10.0 ** a).float()
+    ws = (0.5 + torch.rand(N, generator=g, device="cuda", dtype=torch.float64)).mul(10.0 ** b).float()
+    assert torch.isfinite(s).all() and torch.isfinite(ws).all()
+    cases = [(ops.QuantRows(q, s), q, s)]
+    x = (q.double() * s.double()[:, None]).float()
+    if torch.isfinite(x).all():
+        cases.append((x, *ops.quantize_rows(x)))
+    top = float(torch.finfo(torch.float32).max)
+    for rows, codes, scale in cases:
+        for relu in (False, True):
+            y = ops.int8_linear(rows, ops.QuantRows(w, ws), relu=relu)
+            want, _ = int8_plain(codes, scale, w, ws, None)
+            if relu:
+                want = want.clamp_min(0)
+            sure = want.abs() * (1 + INT8_SLACK) < top
+            assert (y[want == 0] == 0).all()
+            assert ((y.double() - want).abs()[sure] <= (INT8_SLACK * want.abs() + 2.0 ** -149)[sure]).all()
+            assert torch.isinf(y[want.abs() * (1 - INT8_SLACK) > top]).all() and (torch.sign(y.double()) == torch.sign(want))[~sure].all()
