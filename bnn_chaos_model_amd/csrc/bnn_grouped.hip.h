@@ -425,14 +425,13 @@ __global__ __launch_bounds__(512) void bnn_grouped_few_kernel(RowsParams p) {
         }
         float v[4] = {0, 0, 0, 0};
         if (!nobody) {
-            Scale xs, ws;
-            if constexpr (sizeof(T) == 1) xs = Scale(p.xs[src]);
+            float ws[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) ws[i] = sizeof(T) == 1 ? p.ws[(int64_t)rt.g * p.N + min(n + i, p.N - 1)] : 1.0f;
+            values_of(a, sizeof(T) == 1 ? p.xs[src] : 1.0f, ws, false, v);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int64_t col = (int64_t)rt.g * p.N + min(n + i, p.N - 1);
-                if constexpr (sizeof(T) == 1) ws = Scale(p.ws[col]);
-                v[i] = value_of(a[i], xs, ws);
-                if (p.bias) v[i] += (float)reinterpret_cast<const O*>(p.bias)[col];
+                if (p.bias) v[i] += (float)reinterpret_cast<const O*>(p.bias)[(int64_t)rt.g * p.N + min(n + i, p.N - 1)];
                 if (p.relu) v[i] = v[i] < 0.0f ? 0.0f : v[i];
             }
         }
@@ -468,8 +467,7 @@ __global__ __launch_bounds__(256) void bnn_grouped_short_kernel(RowsParams p) {
     int m = rt.r0 + wave / WN * 16 + i16;
     int pair = place(m), pair1 = place(m + MSTEP);   // (asked for ahead of the matrix: the rows wait for them)
     u32x4 w[FN][ST];
-    float bias[FN][4];
-    Scale ws[FN][4];
+    float bias[FN][4], ws[FN][4];
 #pragma unroll
     for (int j = 0; j < FN; ++j) {
 #pragma unroll
@@ -481,7 +479,7 @@ __global__ __launch_bounds__(256) void bnn_grouped_short_kernel(RowsParams p) {
         for (int i = 0; i < 4; ++i) {
             const int64_t col = (int64_t)(nobody ? 0 : rt.g) * p.N + min(n0 + j * 16 + q * 4 + i, p.N - 1);
             bias[j][i] = p.bias && !nobody ? (float)reinterpret_cast<const O*>(p.bias)[col] : 0.0f;
-            if constexpr (sizeof(T) == 1) ws[j][i] = Scale(nobody ? 1.0f : p.ws[col]);   // (nobody's sums are zero, but zero times a NaN scale is not)
+            ws[j][i] = sizeof(T) == 1 ? p.ws[col] : 1.0f;
         }
     }
     const auto source = [&](int m, int pair) -> int64_t {   // row of x
@@ -489,22 +487,24 @@ __global__ __launch_bounds__(256) void bnn_grouped_short_kernel(RowsParams p) {
         const int o = pair >= 0 && pair < p.P ? pair : 0;
         return p.gather_div > 1 ? o / p.gather_div : o;
     };
-    const auto fetch = [&](int64_t src, u32x4 (&x)[ST]) {
+    const auto fetch = [&](int64_t src, u32x4 (&x)[ST], float& xs) {
         const char* row = p.x + src * p.ldx;
+        if constexpr (sizeof(T) == 1) xs = p.xs[src];   // (with the row: asked for in front of the output it is waited for there)
 #pragma unroll
         for (int s = 0; s < ST; ++s) {
             const int at = s * STEP + q * CHUNK;
             x[s] = load_chunk<T>(row, at, kbytes, (s + 1) * STEP <= kbytes);
         }
     };
-    int64_t src = source(m, pair);
     u32x4 x[ST];
-    if (!nobody) fetch(src, x);
+    float xs = 1.0f;
+    if (!nobody) fetch(source(m, pair), x, xs);
     for (; m - i16 < rt.r1; m += MSTEP) {
         u32x4 xn[ST];
+        float xsn = 1.0f;
         const int64_t src1 = source(m + MSTEP, pair1);
         const int pair2 = place(m + 2 * MSTEP);
-        if (!nobody) fetch(src1, xn);
+        if (!nobody) fetch(src1, xn, xsn);
         Acc acc[FN];
 #pragma unroll
         for (int j = 0; j < FN; ++j) acc[j] = Acc{};
@@ -516,20 +516,19 @@ __global__ __launch_bounds__(256) void bnn_grouped_short_kernel(RowsParams p) {
         const int o = p.scatter ? pair : m;
         if (m < rt.r1 && o >= 0 && o < p.P) {
             char* row = p.y + (int64_t)o * p.ldy;
-            Scale xs;
-            if constexpr (sizeof(T) == 1) xs = Scale(nobody ? 1.0f : p.xs[src]);
 #pragma unroll
             for (int j = 0; j < FN; ++j) {
                 float v[4];
+                values_of(acc[j], xs, ws[j], nobody, v);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    v[i] = value_of(acc[j][i], xs, ws[j][i]) + bias[j][i];
+                    v[i] += bias[j][i];
                     if (p.relu) v[i] = v[i] < 0.0f ? 0.0f : v[i];
                 }
                 store4<O>(row, n0 + j * 16 + q * 4, p.N, v, p.vec);
             }
         }
-        pair = pair1; pair1 = pair2; src = src1;
+        pair = pair1; pair1 = pair2; xs = xsn;
 #pragma unroll
         for (int s = 0; s < ST; ++s) x[s] = xn[s];
     }

@@ -260,14 +260,17 @@ __global__ __launch_bounds__(512) void bnn_int8_handful_kernel(RowsParams p, int
         if (o < 0 || o >= p.P) return;
     }
     float v[4] = {0, 0, 0, 0};
-    if (!nobody)
+    if (!nobody) {
+        float ws[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) ws[i] = p.ws[(int64_t)rt.g * p.N + min(n + i, p.N - 1)];
+        values_of(a, sx[i16], ws, false, v);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int64_t col = (int64_t)rt.g * p.N + min(n + i, p.N - 1);
-            v[i] = value_of(a[i], Scale(sx[i16]), Scale(p.ws[col]));
-            if (p.bias) v[i] += (float)reinterpret_cast<const O*>(p.bias)[col];
+            if (p.bias) v[i] += (float)reinterpret_cast<const O*>(p.bias)[(int64_t)rt.g * p.N + min(n + i, p.N - 1)];
             if (p.relu) v[i] = v[i] < 0.0f ? 0.0f : v[i];
         }
+    }
     store4<O>(p.y + o * p.ldy, n, p.N, v, p.vec);
 }
 

@@ -79,6 +79,25 @@ struct Scale {
 };
 __device__ __forceinline__ float value_of(int32_t sum, Scale xs, Scale ws) { return __builtin_amdgcn_ldexpf(sum_f32(sum) * (xs.m * ws.m), xs.e + ws.e); }
 __device__ __forceinline__ float value_of(float sum, Scale, Scale) { return sum; }
+// The same of four neighbours where a wave's few instructions in a row are what counts: plain products first, looked at again if one of the scales' is
+// not an ordinary float (3 000 rows x 40 -> 40 in 8 bits: 6.20 us, taken apart every time 6.45).  nobody: rows whose sums are zero and have no scales (zero
+// times another member's NaN scale is not zero).
+__device__ __forceinline__ void values_of(i32x4 sum, float xs, const float (&ws)[4], bool nobody, float (&v)[4]) {
+    bool ordinary = true;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float s = xs * ws[i];
+        v[i] = sum_f32(sum[i]) * s;
+        ordinary &= __builtin_isnormal(s);
+    }
+    if (!ordinary)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = nobody ? 0.0f : value_of(sum[i], Scale(xs), Scale(ws[i]));
+}
+__device__ __forceinline__ void values_of(tf32x4 sum, float, const float (&)[4], bool, float (&v)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = sum[i];
+}
 
 // ---- 16-byte loads of rows with any alignment and any length -------------------------------------------------------------------------
 struct __attribute__((packed, aligned(1))) Bytes16 { u32x4 v; };
