@@ -101,6 +101,13 @@ __global__ __launch_bounds__(256) void bnn_group_scan_kernel(int32_t* __restrict
     if (threadIdx.x == 0) total[blockIdx.x] = carry;
 }
 
+// Between lanes of one wave that hand values to each other through LDS: what is read and written before comes before what follows.  A wave's LDS accesses
+// are carried out in order, so this costs nothing; it holds the compiler to that order.
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
 // SINGLE: one workgroup holds every pair (no count and scan launches in front)
 template <int WAVES, bool SINGLE>
 __global__ __launch_bounds__(WAVES * 64) void bnn_group_place_kernel(const int32_t* __restrict__ member, int64_t P, int G, const int32_t* __restrict__ cnt,
@@ -161,9 +168,10 @@ __global__ __launch_bounds__(WAVES * 64) void bnn_group_place_kernel(const int32
             const int before = __popcll(same & ((1ull << lane) - 1));
             const int32_t at = wc[wave * G1 + key];
             order[at + before] = (int32_t)keys.pair(lo, i);
-            if (before == 0) wc[wave * G1 + key] = at + __popcll(same);   // (every lane of the wave has read `at`: one wave runs in step)
+            wave_sync();   // every lane of the wave has read `at` ...
+            if (before == 0) wc[wave * G1 + key] = at + __popcll(same);
         }
-        __builtin_amdgcn_wave_barrier();
+        wave_sync();       // ... and reads what its first one has written
     }
 }
 
