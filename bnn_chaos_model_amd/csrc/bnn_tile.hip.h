@@ -36,14 +36,12 @@ template <> struct Mma<__bf16> {
     static __device__ __forceinline__ Acc mul(u32x4 a, u32x4 b, Acc c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
     }
-    static __device__ __forceinline__ u32x4 ones() { return u32x4{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u}; }
 };
 template <> struct Mma<_Float16> {
     using Acc = tf32x4;
     static __device__ __forceinline__ Acc mul(u32x4 a, u32x4 b, Acc c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
     }
-    static __device__ __forceinline__ u32x4 ones() { return u32x4{0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u}; }
 };
 template <> struct Mma<float> {   // k = 4 q + j goes into instruction j from lane group q: the same order for both operands
     using Acc = tf32x4;
@@ -53,7 +51,6 @@ template <> struct Mma<float> {   // k = 4 q + j goes into instruction j from la
         for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[j], y[j], c, 0, 0, 0);
         return c;
     }
-    static __device__ __forceinline__ u32x4 ones() { return u32x4{0x3f800000u, 0x3f800000u, 0x3f800000u, 0x3f800000u}; }
 };
 template <> struct Mma<int8_t> {
     using Acc = i32x4;
