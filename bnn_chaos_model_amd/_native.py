@@ -141,6 +141,8 @@ def lib():
         f.restype = C.c_size_t
     L.bnn_relu_grad.argtypes = [_vp, C.c_int64, _vp, C.c_int64, C.c_int64, C.c_int32, C.c_int32, _vp, _vp]
     L.bnn_quantize_rows.argtypes = [_vp, C.c_int32, C.c_int64, C.c_int32, C.c_int64, _vp, C.c_int64, _vp, _vp]
+    L.bnn_grouped_linear_form.argtypes = [G, C.c_int32, _vp, _vp, _vp, _vp]
+    L.bnn_int8_linear_form.argtypes = [G, _vp, _vp, _vp, _vp]
     L.bnn_int8_linear.argtypes = [G, _vp, _vp, _vp, _vp, _vp, _vp, _vp]
     if L.bnn_abi_version() != ABI_VERSION:
         raise NativeError(-1, f"ABI version mismatch: {SO_PATH} reports {L.bnn_abi_version()}, this binding is written for {ABI_VERSION}")
@@ -156,7 +158,7 @@ EXPORTS = ("bnn_abi_version", "bnn_last_error", "bnn_device_count", "bnn_param_c
            "bnn_plan_spec_attached", "bnn_spec_embedded_source", "bnn_gen_params_bytes", "bnn_nonfinite_record_bytes", "bnn_nonfinite_scan_f32",
            "bnn_group_rows_workspace_bytes", "bnn_group_rows_i32", "bnn_grouped_linear", "bnn_grouped_linear_dx_workspace_bytes", "bnn_grouped_linear_dx",
            "bnn_grouped_linear_dw_workspace_bytes", "bnn_grouped_linear_dw", "bnn_relu_grad", "bnn_quantize_rows", "bnn_int8_linear",
-           "bnn_int8_linear_rows_workspace_bytes", "bnn_int8_linear_rows")
+           "bnn_int8_linear_rows_workspace_bytes", "bnn_int8_linear_rows", "bnn_grouped_linear_form", "bnn_int8_linear_form")
 
 
 def check(rc):

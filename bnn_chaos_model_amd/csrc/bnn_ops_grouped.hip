@@ -258,9 +258,66 @@ int check_grouped(const bnn_grouped* q) {
     return 0;
 }
 
+RowsParams forward_params(const bnn_grouped* q, const void* x, const void* w, const void* bias, void* y) {
+    const int es = type_size(q->dtype);
+    RowsParams p{};
+    p.x = (const char*)x; p.w = (const char*)w; p.bias = bias; p.y = (char*)y;
+    p.order = q->order; p.offsets = q->offsets;
+    p.ldx = q->x_row * es; p.w_member = q->w_member * es; p.w_row = q->w_row * es; p.ldy = q->y_row * es;
+    p.P = (int32_t)(q->rows * q->copies); p.G = q->members; p.N = q->outputs; p.K = q->inputs;
+    p.gather_div = q->gather ? q->copies : 0; p.scatter = q->scatter ? 1 : 0; p.relu = q->relu ? 1 : 0;
+    return p;
+}
+
+// a row of x fed several pairs: their gradients meet in fp32, one rounding at the end
+bool dx_by_pairs(const bnn_grouped* q) { return q->gather && q->copies > 1; }
+
+RowsParams dx_params(const bnn_grouped* q, const void* dy, const void* w, void* out) {   // out: dx, or the pairs' gradients
+    const int es = type_size(q->dtype);
+    RowsParams p{};
+    p.x = (const char*)dy; p.w = (const char*)w; p.y = (char*)out;
+    p.order = q->order; p.offsets = q->offsets;
+    p.ldx = q->y_row * es; p.w_member = q->w_member * es; p.w_row = q->w_row * es;
+    p.ldy = dx_by_pairs(q) ? (int64_t)q->inputs * sizeof(float) : q->x_row * es;
+    p.P = (int32_t)(q->rows * q->copies); p.G = q->members; p.N = q->inputs; p.K = q->outputs;
+    p.gather_div = q->scatter ? 1 : 0; p.scatter = q->gather ? 1 : 0;
+    return p;
+}
+
+ReduceParams dw_params(const bnn_grouped* q, const void* dy, const void* x, void* dw) {
+    const int es = type_size(q->dtype);
+    ReduceParams p{};
+    p.x = (const char*)x; p.dy = (const char*)dy; p.dw = (char*)dw;
+    p.offsets = q->offsets;
+    p.ldx = (uint32_t)(q->x_row * es); p.lddy = (uint32_t)(q->y_row * es);
+    p.P = (int32_t)(q->rows * q->copies); p.G = q->members; p.N = q->outputs; p.K = q->inputs;
+    p.m_x = q->gather ? -1 : 0; p.m_dy = q->scatter ? -1 : 0;
+    p.list = p.m_x | p.m_dy ? q->order : nullptr;
+    while ((1LL << p.shift) < q->copies) ++p.shift;   // pair / copies = (2 pair * magic >> 32) >> shift, exact below 2^31: magic = ceil(2^(31 + shift) / copies)
+    p.magic = (uint32_t)(((1ULL << (31 + p.shift)) + q->copies - 1) / q->copies);
+    return p;
+}
+
 }  // namespace
 
 extern "C" {
+
+int bnn_grouped_linear_form(const bnn_grouped* q, int32_t pass, const void* a, const void* b, const void* out, int32_t* form) {
+    if (!form || pass < BNN_PASS_FORWARD || pass > BNN_PASS_DW) return fail(BNN_ERR_INVALID, "bad argument");
+    if (int rc = check_grouped(q)) return rc;
+    RowsForm f;
+    int splits = 1;
+    if (pass == BNN_PASS_FORWARD) f = form_of_rows(q->dtype, q->dtype, false, forward_params(q, a, b, nullptr, (void*)out));
+    else if (pass == BNN_PASS_DX) f = form_of_rows(q->dtype, dx_by_pairs(q) ? BNN_TYPE_F32 : q->dtype, true, dx_params(q, a, b, (void*)out));
+    else {
+        const ReducePlan plan = plan_of(q);
+        f = form_of_reduce(q->dtype, dw_params(q, a, b, (void*)out), plan.tile);
+        splits = plan.splits;
+    }
+    const int32_t values[6] = {f.kind, f.rows, f.outputs, f.direct, f.steps, splits};
+    std::copy(values, values + 6, form);
+    return 0;
+}
 
 size_t bnn_group_rows_workspace_bytes(int64_t pairs, int32_t members) {
     if (pairs <= GROUP_CHUNK || members < 1 || members > GROUP_MAX_MEMBERS) return 0;
@@ -309,14 +366,7 @@ int bnn_grouped_linear(const bnn_grouped* q, const void* x, const void* w, const
     if (int rc = check_grouped(q)) return rc;
     if (q->rows == 0) return 0;
     if (!x || !w || !y || !q->offsets) return fail(BNN_ERR_INVALID, "NULL argument");
-    const int es = type_size(q->dtype);
-    RowsParams p{};
-    p.x = (const char*)x; p.w = (const char*)w; p.bias = bias; p.y = (char*)y;
-    p.order = q->order; p.offsets = q->offsets;
-    p.ldx = q->x_row * es; p.w_member = q->w_member * es; p.w_row = q->w_row * es; p.ldy = q->y_row * es;
-    p.P = (int32_t)(q->rows * q->copies); p.G = q->members; p.N = q->outputs; p.K = q->inputs;
-    p.gather_div = q->gather ? q->copies : 0; p.scatter = q->scatter ? 1 : 0; p.relu = q->relu ? 1 : 0;
-    return launch_rows(q->dtype, q->dtype, false, p, (hipStream_t)stream);
+    return launch_rows(q->dtype, q->dtype, false, forward_params(q, x, w, bias, y), (hipStream_t)stream);
 }
 
 size_t bnn_grouped_linear_dx_workspace_bytes(const bnn_grouped* q) {
@@ -328,18 +378,10 @@ int bnn_grouped_linear_dx(const bnn_grouped* q, const void* dy, const void* w, v
     if (int rc = check_grouped(q)) return rc;
     if (q->rows == 0) return 0;
     if (!dy || !w || !dx || !q->offsets) return fail(BNN_ERR_INVALID, "NULL argument");
-    const int es = type_size(q->dtype);
-    const bool pairs = q->gather && q->copies > 1;   // a row of x fed several pairs: their gradients meet in fp32, one rounding at the end
+    const bool pairs = dx_by_pairs(q);
     if (pairs && !workspace) return fail(BNN_ERR_INVALID, "workspace is NULL");
     if (pairs && q->x_row != q->inputs) return fail(BNN_ERR_INVALID, "dx of several copies must be dense");
-    RowsParams p{};
-    p.x = (const char*)dy; p.w = (const char*)w; p.y = pairs ? (char*)workspace : (char*)dx;
-    p.order = q->order; p.offsets = q->offsets;
-    p.ldx = q->y_row * es; p.w_member = q->w_member * es; p.w_row = q->w_row * es;
-    p.ldy = pairs ? (int64_t)q->inputs * sizeof(float) : q->x_row * es;
-    p.P = (int32_t)(q->rows * q->copies); p.G = q->members; p.N = q->inputs; p.K = q->outputs;
-    p.gather_div = q->scatter ? 1 : 0; p.scatter = q->gather ? 1 : 0;
-    if (int rc = launch_rows(q->dtype, pairs ? BNN_TYPE_F32 : q->dtype, true, p, (hipStream_t)stream)) return rc;
+    if (int rc = launch_rows(q->dtype, pairs ? BNN_TYPE_F32 : q->dtype, true, dx_params(q, dy, w, pairs ? workspace : dx), (hipStream_t)stream)) return rc;
     if (!pairs) return 0;
     const auto join = [&](auto tag) -> int {
         using O = typename decltype(tag)::type;
@@ -367,16 +409,8 @@ size_t bnn_grouped_linear_dw_workspace_bytes(const bnn_grouped* q) {
 int bnn_grouped_linear_dw(const bnn_grouped* q, const void* dy, const void* x, void* dw, void* db, void* workspace, void* stream) {
     if (int rc = check_grouped(q)) return rc;
     if (!dw || !q->offsets || (q->rows && (!dy || !x))) return fail(BNN_ERR_INVALID, "NULL argument");
-    const int es = type_size(q->dtype);
-    ReduceParams p{};
-    p.x = (const char*)x; p.dy = (const char*)dy; p.dw = (char*)dw; p.db = db; p.part = (float*)workspace;
-    p.offsets = q->offsets;
-    p.ldx = (uint32_t)(q->x_row * es); p.lddy = (uint32_t)(q->y_row * es);
-    p.P = (int32_t)(q->rows * q->copies); p.G = q->members; p.N = q->outputs; p.K = q->inputs;
-    p.m_x = q->gather ? -1 : 0; p.m_dy = q->scatter ? -1 : 0;
-    p.list = p.m_x | p.m_dy ? q->order : nullptr;
-    while ((1LL << p.shift) < q->copies) ++p.shift;   // pair / copies = (2 pair * magic >> 32) >> shift, exact below 2^31: magic = ceil(2^(31 + shift) / copies)
-    p.magic = (uint32_t)(((1ULL << (31 + p.shift)) + q->copies - 1) / q->copies);
+    ReduceParams p = dw_params(q, dy, x, dw);
+    p.db = db; p.part = (float*)workspace;
     const ReducePlan plan = plan_of(q);
     p.splits = q->rows ? plan.splits : 1;
     if (p.splits > 1 && (!workspace || (uintptr_t)workspace % 16)) return fail(BNN_ERR_INVALID, "workspace is NULL or not 16-byte aligned");

@@ -336,6 +336,22 @@ int bnn_quantize_rows(const void* x, int32_t dtype, int64_t rows, int32_t K, int
     return dtype == BNN_TYPE_BF16 ? launch(Tag<__bf16>{}) : launch(Tag<_Float16>{});
 }
 
+int bnn_int8_linear_form(const bnn_grouped* q, const int8_t* x, const int8_t* w, const void* y, int32_t* form) {
+    if (!form) return fail(BNN_ERR_INVALID, "bad argument");
+    if (int rc = check_int8(q)) return rc;
+    RowsParams p = int8_params(q, w, nullptr, nullptr, (void*)y);
+    p.x = (const char*)x; p.ldx = q->x_row;
+    const auto of = [&](auto tag) {
+        using O = typename decltype(tag)::type;
+        set_vec<O>(p);
+        return rows_form<int8_t, O, false>(p);
+    };
+    const RowsForm f = q->dtype == BNN_TYPE_F32 ? of(Tag<float>{}) : q->dtype == BNN_TYPE_BF16 ? of(Tag<__bf16>{}) : of(Tag<_Float16>{});
+    const int32_t values[6] = {f.kind, f.rows, f.outputs, f.direct, f.steps, 1};
+    std::copy(values, values + 6, form);
+    return 0;
+}
+
 int bnn_int8_linear(const bnn_grouped* q, const int8_t* x, const float* x_scale, const int8_t* w, const float* w_scale, const void* bias, void* y,
                     void* stream) {
     if (int rc = check_int8(q)) return rc;
@@ -370,7 +386,7 @@ int bnn_int8_linear_rows(const bnn_grouped* q, const void* x, int32_t x_dtype, v
         const auto launch = [&](auto xt, auto ot) -> int {
             using XT = typename decltype(xt)::type;
             using O = typename decltype(ot)::type;
-            p.vec = p.N % 4 == 0 && aligned(p.ldy, 4 * sizeof(O)) && aligned(p.y, 4 * sizeof(O));
+            set_vec<O>(p);
             if (int rc = set_grid(p, 16, 16, 1, 512)) return rc;
             constexpr auto* kern = &bnn_int8_handful_kernel<XT, O>;
             allow_big_lds<kern>();

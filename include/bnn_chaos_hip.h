@@ -390,6 +390,15 @@ size_t bnn_grouped_linear_dw_workspace_bytes(const bnn_grouped* q);
 int bnn_grouped_linear_dw(const bnn_grouped* q, const void* dy, const void* x, void* dw, void* db, void* workspace, void* stream);
 int bnn_relu_grad(const void* dy, int64_t dy_row, const void* y, int64_t y_row, int64_t rows, int32_t N, int32_t dtype, void* out, void* stream);
 
+/* Which kernel a call of these runs, by the rules on sizes, types and alignment (host only, nothing is enqueued; lets a test see that its sizes reach a
+ * kernel).  a, b, out: the addresses of the pass, of which the alignment counts alone: forward x, w, y; dx dy, w and dx (or its workspace, with gather and
+ * copies > 1); dw dy, x, dw.  form receives kind, rows and outputs of a workgroup (dw: outputs and inputs), whether rows are loaded in whole aligned
+ * 16-byte chunks, 64-byte steps of a short row, parts that the rows of a member are split into (dw). */
+enum bnn_grouped_pass { BNN_PASS_FORWARD = 0, BNN_PASS_DX = 1, BNN_PASS_DW = 2 };
+enum bnn_grouped_kind { BNN_GROUPED_FEW = 0, BNN_GROUPED_SHORT = 1, BNN_GROUPED_TILE = 2, BNN_GROUPED_DW = 3, BNN_GROUPED_DW_LISTED = 4 };
+int bnn_grouped_linear_form(const bnn_grouped* q, int32_t pass, const void* a, const void* b, const void* out, int32_t form[6]);
+int bnn_int8_linear_form(const bnn_grouped* q, const int8_t* x, const int8_t* w, const void* y, int32_t form[6]);   /* of bnn_int8_linear */
+
 /* 8-bit operands.  bnn_quantize_rows: scale = max |x| / 127 of the row, q = x / scale rounded half to even -- the exact quotient's rounding,
  * not that of a rounded reciprocal.  A row of zeros has scale 0; a row that holds NaN or +-inf has scale NaN and codes 0, so that everything
  * computed from it is NaN.  q rows are q_row >= K bytes apart and zero behind K.

@@ -1,11 +1,13 @@
 """CPU: what the linear layers over row groups check before they call a kernel -- groups that a caller has altered, operands whose derivative would be lost."""
 import copy
+import ctypes as C
 
 import pytest
 import torch
 from torch.autograd import forward_ad
 from torch.utils import _pytree
 
+from bnn_chaos_model_amd import _native as N
 from bnn_chaos_model_amd import member_linear as M
 from bnn_chaos_model_amd import ops
 
@@ -99,3 +101,60 @@ def test_operands_with_a_tangent_are_refused(i):
             call(forward_ad.make_dual(t, torch.ones_like(t)))
         with pytest.raises(TypeError):       # a plain operand next to a dual level: the next check (these are on the CPU)
             call(t)
+
+
+# ---- the kernels that the tests reach --------------------------------------------------------------------------------------------------------
+FEW, SHORT, TILE, DW, DW_LISTED = range(5)   # (bnn_grouped_kind)
+
+
+def form(fn, q, *args):
+    out = (C.c_int32 * 6)()
+    assert fn(C.byref(q), *args, out) == 0
+    return tuple(out)
+
+
+def forms(rows, members, copies, K, No, dtype, moved):
+    """{(pass, bytes of an operand's element): what it runs} for dense operands as torch allocates them (addresses of whole 512 bytes)."""
+    L, es, c = N.lib(), 4 if dtype == 0 else 2, max(copies, 1)
+    q = N.BnnGrouped(rows, c, members, K, No, dtype, moved, moved, 0, K, No, No * K, K, 512, 512)
+    out = {("forward", es): form(L.bnn_grouped_linear_form, q, 0, 512, 512, 512), ("dx of copies" if c > 1 and moved else "dx", es): form(L.bnn_grouped_linear_form, q, 1, 512, 512, 512),
+           ("dw", es): form(L.bnn_grouped_linear_form, q, 2, 512, 512, 512), ("int8", 1): form(L.bnn_int8_linear_form, q, 512, 512, 512)}
+    return out
+
+
+def test_the_sizes_reach_every_kernel():
+    from test_member_linear_forms import SIZES
+    got = set()
+    for (n, G, c, K, No) in SIZES:
+        for dtype in (0, 1):
+            for moved in (1, 0):
+                for (what, es), (kind, rows, outputs, direct, steps, splits) in forms(n, G, c, K, No, dtype, moved).items():
+                    if kind == TILE and (No if what.startswith("dx") else K) * es <= 4 * 128:
+                        continue    # (at least five stages, so that the loop turns)
+                    got.add((what, es, kind, rows, outputs, direct, steps, splits > 1))
+    tiles = [(64, 64, 0), (64, 64, 1), (128, 128, 0), (128, 128, 1), (256, 256, 1)]
+    want = set()
+    for what, es in (("forward", 4), ("forward", 2), ("int8", 1)):
+        want |= {(what, es, FEW, r, o, d, 0, False) for r, o in ((16, 16), (16, 32), (32, 32)) for d in (0, 1)}
+        want |= {(what, es, SHORT, r, o, 0, s, False) for r, o in ((64, 64), (64, 128), (128, 128)) for s in (1, 2, 3, 4)}
+        want |= {(what, es, TILE, r, o, d, 0, False) for r, o, d in tiles}
+    want |= {("int8", 1, TILE, 256, 128, 0, 0, False), ("forward", 4, SHORT, 128, 64, 0, 3, False), ("int8", 1, SHORT, 128, 64, 0, 1, False)}
+    for what in ("dx", "dx of copies"):
+        want |= {(what, es, TILE, r, o, d, 0, False) for es in (4, 2) for r, o, d in tiles}
+    for kind in (DW, DW_LISTED):
+        want |= {("dw", es, kind, t, t, d, 0, False) for es in (4, 2) for t in (64, 128) for d in (0, 1)} | {("dw", 2, kind, 256, 256, 1, 0, False)}
+        want |= {("dw", es, kind, 64, 64, d, 0, True) for es in (4, 2) for d in (0, 1)}
+    assert not want - got, sorted(want - got)
+    assert not {f for f in got if f not in want and f[2] != SHORT}      # a form that is new must be written down here
+
+
+def test_form_refuses_what_the_calls_refuse():
+    L, out = N.lib(), (C.c_int32 * 6)()
+    q = N.BnnGrouped(4, 1, 2, 8, 3, 0, 0, 0, 0, 8, 3, 24, 8, None, 1)
+    for p in (-1, 3):
+        assert L.bnn_grouped_linear_form(C.byref(q), p, 16, 16, 16, out) == N.ERR_INVALID
+    assert L.bnn_grouped_linear_form(C.byref(q), 0, 16, 16, 16, None) == L.bnn_int8_linear_form(C.byref(q), 16, 16, 16, None) == N.ERR_INVALID
+    q.copies = 0
+    assert L.bnn_grouped_linear_form(C.byref(q), 0, 16, 16, 16, out) == L.bnn_int8_linear_form(C.byref(q), 16, 16, 16, out) == N.ERR_INVALID
+    empty = N.BnnGrouped(0, 1, 2, 8, 3, 0, 0, 0, 0, 8, 3, 24, 8, None, 1)
+    assert all(L.bnn_grouped_linear_form(C.byref(empty), p, 16, 16, 16, out) == 0 for p in range(3))
