@@ -61,13 +61,11 @@ def _addr(t):
 
 
 def _rows2d(t):
-    """t [n, K] with its elements side by side in a row; rows may be any distance apart (a slice, an expanded row)."""
-    row, col = t.stride()
-    return t if (col == 1 or t.shape[1] <= 1) and row <= 1 << 28 else t.contiguous()
-
-
-def _row_stride(t):
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    """t [n, K] with its elements side by side in a row, and how many elements its rows are apart (any distance: a slice, an expanded row)."""
+    (row, col), (n, k) = t.stride(), t.shape
+    if (col != 1 and k > 1) or row > 1 << 28:
+        t, row = t.contiguous(), k
+    return t, row if n > 1 else k
 
 
 def _layers(w):
@@ -164,11 +162,12 @@ def _descriptor(groups, rows, copies, dtype, weight, x_row, y_row, gather, scatt
 
 
 def _linear(x, weight, groups, bias, relu, gather, scatter, rows, copies):
-    x, weight = _rows2d(x), _layers(weight)
+    (x, x_row), weight = _rows2d(x), _layers(weight)
     if bias is not None and not bias.is_contiguous():
         bias = bias.contiguous()
-    y = x.new_empty(_out_shape(groups, rows * copies, weight.shape[1], scatter))
-    q = _descriptor(groups, rows, copies, x.dtype, weight, _row_stride(x), weight.shape[1], gather, scatter, relu)
+    n_out = weight.shape[1]
+    y = x.new_empty(_out_shape(groups, rows * copies, n_out, scatter))
+    q = _descriptor(groups, rows, copies, x.dtype, weight, x_row, n_out, gather, scatter, relu)
     _run(x.get_device(), N.lib().bnn_grouped_linear, q, x.data_ptr(), weight.data_ptr(), _addr(bias), y.data_ptr())
     return y
 
@@ -191,26 +190,26 @@ def grouped_linear_grads(dy, x, weight, groups, y=None, gather=False, scatter=Fa
         if tuple(t.shape) != shape:
             raise ValueError(f"{name} must be {list(shape)}")
         _same_device(dev, name, t)
-    x, weight = _rows2d(x), _layers(weight)
-    dy = _rows2d(dy.reshape(-1, n_out))
+    (x, x_row), weight = _rows2d(x), _layers(weight)
+    dy, dy_row = _rows2d(dy.reshape(-1, n_out))
     need_x, need_w, need_b = need
     L = N.lib()
     if y is not None:
-        y2 = _rows2d(y.reshape(-1, n_out))
+        y2, y_row = _rows2d(y.reshape(-1, n_out))
         masked = x.new_empty((dy.shape[0], n_out))
-        _run(dev, L.bnn_relu_grad, dy.data_ptr(), _row_stride(dy), y2.data_ptr(), _row_stride(y2), dy.shape[0], n_out, _TYPES[x.dtype], masked.data_ptr())
-        dy = masked
+        _run(dev, L.bnn_relu_grad, dy.data_ptr(), dy_row, y2.data_ptr(), y_row, dy.shape[0], n_out, _TYPES[x.dtype], masked.data_ptr())
+        dy, dy_row = masked, n_out
     dx = dw = db = None
     if need_x:
         dx = x.new_empty((x.shape[0], n_in))
-        q = _descriptor(groups, rows, copies, x.dtype, weight, n_in, _row_stride(dy), gather, scatter)
+        q = _descriptor(groups, rows, copies, x.dtype, weight, n_in, dy_row, gather, scatter)
         nbytes = L.bnn_grouped_linear_dx_workspace_bytes(q)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
         _run(dev, L.bnn_grouped_linear_dx, q, dy.data_ptr(), weight.data_ptr(), dx.data_ptr(), _addr(ws))
     if need_w or need_b:
         dw = x.new_empty((G, n_out, n_in))
         db = x.new_empty((G, n_out)) if need_b else None
-        q = _descriptor(groups, rows, copies, x.dtype, weight, _row_stride(x), _row_stride(dy), gather, scatter)
+        q = _descriptor(groups, rows, copies, x.dtype, weight, x_row, dy_row, gather, scatter)
         nbytes = L.bnn_grouped_linear_dw_workspace_bytes(q)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
         _run(dev, L.bnn_grouped_linear_dw, q, dy.data_ptr(), x.data_ptr(), dw.data_ptr(), _addr(db), _addr(ws))
@@ -273,10 +272,10 @@ def quantize_rows(x):
     _check_quantize(x)
     shape = x.shape
     K = shape[-1]
-    x2 = _rows2d(x if len(shape) == 2 else x.reshape(-1, K))
+    x2, x_row = _rows2d(x if len(shape) == 2 else x.reshape(-1, K))
     values = torch.empty(shape, dtype=torch.int8, device=x.device)
     scale = torch.empty(shape[:-1], dtype=torch.float32, device=x.device)
-    _run(x.get_device(), N.lib().bnn_quantize_rows, x2.data_ptr(), _TYPES[x.dtype], x2.shape[0], K, _row_stride(x2), values.data_ptr(), K, scale.data_ptr())
+    _run(x.get_device(), N.lib().bnn_quantize_rows, x2.data_ptr(), _TYPES[x.dtype], x2.shape[0], K, x_row, values.data_ptr(), K, scale.data_ptr())
     return QuantRows(values, scale)
 
 
@@ -342,9 +341,9 @@ def int8_linear(x, weight, groups=None, bias=None, relu=False, gather=False, sca
         rows, copies = _check_groups(groups, rows_of, G, gather)
         order, offsets = groups.order.data_ptr(), groups.offsets.data_ptr()
         out = _out_shape(groups, rows * copies, n_out, scatter)
-    rows_of, ws = _rows2d(rows_of), ws.contiguous()
+    (rows_of, x_row), ws = _rows2d(rows_of), ws.contiguous()
     y = rows_of.new_empty(out, dtype=dtype)
-    q = N.BnnGrouped(rows, copies, G, n_in, n_out, _TYPES[dtype], 1 if gather else 0, 1 if scatter else 0, 1 if relu else 0, _row_stride(rows_of), n_out,
+    q = N.BnnGrouped(rows, copies, G, n_in, n_out, _TYPES[dtype], 1 if gather else 0, 1 if scatter else 0, 1 if relu else 0, x_row, n_out,
                      strides[0] if G > 1 else 0, strides[1] if n_out > 1 else n_in, order, offsets)
     if quant:
         _same_device(dev, "x.scale", xs)
