@@ -208,8 +208,8 @@ __device__ __forceinline__ void store4(char* row, int n, int N, const float v[4]
 
 // ---- forward / dX --------------------------------------------------------------------------------------------------------------------------
 // Y = X W^T (or dX = dY W) of a member's rows.  Bound by the matrix pipe from a few hundred rows a member on: a 256 x 256 tile does 64 products per byte it
-// loads in 16 bits.  Measured: 65 536 pairs x 4 096 -> 4 096 bf16 in 1.87 ms (1.17 PFLOP/s; matrix pipe 62-66 % busy), 16 384 x 4 096 -> 8 192 in 8 bits
-// 0.49-0.57 ms (1.9-2.2 POP/s).
+// loads in 16 bits.  Measured, launches back to back: 65 536 pairs x 4 096 -> 4 096 bf16 in 1.84 ms (1.20 PFLOP/s; matrix pipe 62-66 % busy), 16 384 x 4 096 -> 8 192
+// in 8 bits 0.47 ms (2.3 POP/s).  The first 20 or so launches after a pause take up to a quarter longer, until the clock has settled.
 // BM rows x BN outputs per workgroup, WM x WN waves.  WFC: the matrix is used the other way round (element (k, n) at k * w_row + n): dX.
 template <typename T, typename O, int BM, int BN, int WM, int WN, bool WFC, bool DMA>
 __device__ __forceinline__ void grouped_tile(const RowsParams& p, const RowTile rt, const int tn, char* smem) {
@@ -346,7 +346,7 @@ __global__ __launch_bounds__(WM * WN * 64, WM * WN * 64 >= 512 ? 2 : 1) void bnn
 // ---- forward of few rows --------------------------------------------------------------------------------------------------------------------
 // 16 FM rows x 16 FN outputs per workgroup of eight waves.  With few rows per member the matrices are what is read: nothing is shared through LDS,
 // every wave takes an eighth of the reduction and loads fragments of W and x as they lie in memory (64 bytes of 16 rows per load, U steps in
-// flight), and the eight partial sums meet in LDS, in the waves' order.  Bound by the latency of a wave's loads: 15 rows of 30 members, 40 -> 40 fp32, 5.6 us.
+// flight), and the eight partial sums meet in LDS, in the waves' order.  Bound by the latency of a wave's loads: 15 rows of 30 members, 40 -> 40 fp32, 5.4 us.
 template <typename T, typename O, int FM, int FN, int U, bool VEC>
 __global__ __launch_bounds__(512) void bnn_grouped_few_kernel(RowsParams p) {
     constexpr int WAVES = 8, BM = 16 * FM, BN = 16 * FN, STEP = 64;
@@ -443,7 +443,7 @@ __global__ __launch_bounds__(512) void bnn_grouped_few_kernel(RowsParams p) {
 // Rows of up to 64 ST bytes: the member's matrix stays in registers, FN x ST fragments a wave, while `block_rows` rows of the batch stream by,
 // sixteen at a time -- no LDS, no barrier; what is read and written is the batch.  WN of the four waves share a row (each 16 FN outputs; its second
 // to fourth reading comes from the first-level cache), so that a wave's part of the matrix is small and many waves fit.  The rows' places are
-// fetched two steps ahead and the rows one step ahead of their products.  150 000 x 41 -> 128 fp32: 43 us (2.3 TB/s); its products alone would take 10-12,
+// fetched two steps ahead and the rows one step ahead of their products.  150 000 x 41 -> 128 fp32: 44 us (2.3 TB/s); its products alone would take 10-12,
 // writing alone takes 14, so what is left is the latency of a row's way.
 template <typename T, typename O, int FN, int ST, int WN>
 __global__ __launch_bounds__(256) void bnn_grouped_short_kernel(RowsParams p) {
@@ -551,8 +551,9 @@ __device__ __forceinline__ int largest_member(const int32_t* __restrict__ off, i
 }
 
 // ---- dW, db --------------------------------------------------------------------------------------------------------------------------------
-// dW = dY^T X over a member's rows.  Bound by the matrix pipe where the member has a few hundred rows: 32 768 rows of 16 members, 2 048 x 2 048 bf16, 305 us
-// with the bias (0.90 PFLOP/s).  Few tiles (30 000 rows of 30 members, 128 x 128 fp32: 120) would leave most CUs idle: their rows are split, 34 + 4 us.
+// dW = dY^T X over a member's rows.  Bound by the matrix pipe where the member has a few hundred rows: 32 768 rows of 16 members, 2 048 x 2 048 bf16, 260 us
+// with the bias (1.06 PFLOP/s).  Few tiles (30 000 rows of 30 members, 128 x 128 fp32: 120) would leave most CUs idle: their rows are split, 33 + 4 us.
+// Every member's rows are cut into as many parts, so that the largest member is last where members are uneven.
 // BT outputs x BT inputs of one member per workgroup, over split blockIdx.y of the member's rows; further workgroups sum dy's columns, the bias
 // gradient.
 // LISTED: rows of x or dy are found through the order (else both are in grouped order, and a load's row is the wave's plus a constant).

@@ -15,7 +15,7 @@ using namespace bnn;
 // One wave takes 64 consecutive pairs at a time, in order: the lanes that hold the same member are found with one ballot per bit of the key, a
 // lane's place is the number of such lanes before it, and the wave's running count per member lives in LDS.  Pairs of nobody (member outside
 // [0, G)) take key G and come last.  Counts per (member, block), their prefix sums, then places; up to GROUP_CHUNK pairs one workgroup does it
-// all.  A thread's keys are loaded at once and stay in registers.  Measured: 3 000 pairs of 30 members 4.7 us, 4 M pairs 5.6 + 3.0 + 16.8 (32 MB read and
+// all.  A thread's keys are loaded at once and stay in registers.  Measured: 3 000 pairs of 30 members 4.5 us, 4 M pairs 5.7 + 3.0 + 17.3 (32 MB read and
 // 16 MB written would take 10): bound by the chain of count, prefix and place in every workgroup.
 constexpr int GROUP_CHUNK = 4096;      // pairs per workgroup
 constexpr int GROUP_MAX_MEMBERS = 4096;

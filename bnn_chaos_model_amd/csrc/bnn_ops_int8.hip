@@ -63,7 +63,7 @@ template <int E> struct __attribute__((packed, aligned(1))) Codes { uint32_t w[E
 
 // Largest magnitude of a row, then its codes.  TPR threads take a row, in chunks of 16 bytes; the first HELD chunks of a thread stay in registers
 // between the two sweeps, longer rows are read again.  Rows are at least one chunk long.
-// Bound by memory: 65 536 x 4 096 bf16 read once, 8-bit codes written once, 163 us (4.9 TB/s).
+// Bound by memory: 65 536 x 4 096 bf16 read once, 8-bit codes written once, 165 us (4.9 TB/s).
 template <typename T, int TPR>
 __global__ __launch_bounds__(256) void bnn_quantize_rows_kernel(const char* __restrict__ x, int64_t ldx, int64_t rows, int K, int8_t* __restrict__ q, int64_t ldq,
                                                                 float* __restrict__ scale) {
@@ -163,7 +163,7 @@ __global__ __launch_bounds__(256) void bnn_quantize_short_rows_kernel(const char
 
 // The layer for a handful of rows in one launch: a workgroup of eight waves quantises the (up to 16) rows of its tile into LDS -- every workgroup
 // again: that is a few kilobytes from L2 against a launch -- while its first fragments of the matrix are on their way, then goes on like
-// bnn_grouped_few_kernel: an eighth of the reduction per wave, partial sums joined in LDS.  Bound by latency: one row of 4 096 -> 4 096, 7.9 us (its matrix
+// bnn_grouped_few_kernel: an eighth of the reduction per wave, partial sums joined in LDS.  Bound by latency: one row of 4 096 -> 4 096, 8.2 us (its matrix
 // alone: 3.5).
 template <typename XT, typename O>
 __global__ __launch_bounds__(512) void bnn_int8_handful_kernel(RowsParams p, int ldq) {

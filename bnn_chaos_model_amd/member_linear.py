@@ -178,7 +178,9 @@ def grouped_linear_grads(dy, x, weight, groups, y=None, gather=False, scatter=Fa
     dy: gradient of the layer's output, in its shape; y: that output, for a layer with relu=True (no gradient where y <= 0; a NaN output passes it, as in
     nn.ReLU), else None.
     A plain function without autograd: what grouped_linear's backward calls, and what a captured HIP graph of a training step may call.
-    dweight and dbias of a member without rows are zero; sums are fp32 and do not depend on timing."""
+    dweight and dbias of a member without rows are zero; sums are fp32 and do not depend on timing.
+    Memory for the call: with gather and several copies dx takes rows x copies x K floats (a row's gradients meet in fp32), with y a masked copy of dy, and
+    dbias is computed along with dweight."""
     if forward_ad._current_level >= 0:
         _no_tangents(dy=dy, y=y)
     rows, copies = _check_linear(x, weight, groups, None, gather)
@@ -241,6 +243,7 @@ def grouped_linear(x, weight, groups, bias=None, relu=False, gather=False, scatt
     scatter=True: y comes in the batch's order, [rows, N] or [rows, copies, N]; False: in grouped order, [pairs, N] -- so a chain of layers
     gathers in the first, scatters in the last and permutes nothing in between.  Rows of nobody: zero.
     Under stream capture call it in torch.no_grad() (a captured training step: grouped_linear_grads for its backward pass).
+    Forward-mode derivatives are refused.
     x and weight may be strided as long as the elements along K are neighbours (a layer's slice of flat parameter vectors [members, d]).
     Sums are fp32 (float32 operands: exact fp32 products), rounded once to the operands' type."""
     rows, copies = _check_linear(x, weight, groups, bias, gather)

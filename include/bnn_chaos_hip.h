@@ -367,9 +367,10 @@ int bnn_multiswag_bands_f32(const bnn_plan* plan, const bnn_grid* grid, const fl
  * gather = 1: x (and dx) holds the batch's `rows` rows and grouped row r reads row order[r] / copies; 0: it holds rows * copies rows in grouped
  * order.  scatter = 1: y (and dy) is in pair order; 0: in grouped order.  order is a permutation of the pairs (only read with gather or
  * scatter; entries out of range are skipped), offsets ascend; both are device pointers.  y / dx rows are written exactly once, rows between them
- * (x_row > inputs) are not touched.  x, w, bias, y share `dtype`; sums are fp32, one rounding at the end.
+ * (x_row > inputs) are not touched; what is written (y, dx) has y_row >= outputs and x_row >= inputs, what is read may overlap.  x, w, bias, y share `dtype`; sums are fp32, one rounding at the end.
  *   bnn_grouped_linear      y  = act(W x + b), act = ReLU with relu = 1 (NaN stays NaN); bias [members, outputs] dense or NULL
- *   bnn_grouped_linear_dx   dx = W^T dy, the copies of a row added in order (fp32 workspace: bnn_grouped_linear_dx_workspace_bytes)
+ *   bnn_grouped_linear_dx   dx = W^T dy, the copies of a row added in order (with gather and copies > 1 an fp32 workspace of rows x copies x inputs:
+ *                           bnn_grouped_linear_dx_workspace_bytes; x_row = inputs then)
  *   bnn_grouped_linear_dw   dw [members, outputs, inputs], db [members, outputs] (or NULL), dense; zero for a member without rows.
  *                           The result depends on the shapes only, not on timing: no atomics.
  *   bnn_relu_grad           out[rows, N] (dense) = 0 where y <= 0, else dy (also where y is NaN): the gradient in front of the two above for a layer with relu = 1 */
