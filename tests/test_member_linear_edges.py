@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 import torch
 
-from test_member_linear import DT, INT8_SLACK, _gen, int8_plain, make, members, ops, pair_view, plain, within  # noqa: F401
+from test_member_linear import INT8_SLACK, _gen, int8_plain, make, ops  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
